@@ -45,7 +45,8 @@ typedef enum rns_status {
     RNS_ERR_UNSUPPORTED = 3,      /* valid request outside what the kernels cover  */
     RNS_ERR_OVERFLOW = 4,         /* P or a dot-product bound exceeds its type     */
     RNS_ERR_CUDA = 5,             /* a CUDA runtime/driver call failed             */
-    RNS_ERR_DEVICE_TIMEOUT = 6    /* a bounded device-side wait expired            */
+    RNS_ERR_DEVICE_TIMEOUT = 6,   /* a bounded device-side wait expired            */
+    RNS_ERR_BAD_INDEX = 7         /* a page index, length or start read on the device is out of range */
 } rns_status;
 
 /* Element type of the source integers handed to the encoders. */
@@ -539,6 +540,124 @@ RNS_API int rns_linear_static(const void* d_x, rns_float_type type, int m, int k
                               const int8_t* d_w_packed, int n, const int32_t* moduli, int channels,
                               const float* d_col_scale, const float* d_bias, void* d_out, int64_t ldo,
                               int32_t out_type, int32_t* d_status, rns_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Paged 8-bit key/value cache and the attention that reads it
+ *
+ * No counterpart in the reference, whose attention stays in floating point
+ * (scripts/evaluate_ppl.py:53-94 replaces the projections around it).
+ * --------------------------------------------------------------------- */
+
+/* What a cached byte stands for, times the block's scale. */
+typedef enum rns_kv_format {
+    RNS_KV_INT8 = 0, /* an integer in [-127, 127]                                  */
+    RNS_KV_E4M3 = 1  /* an 8-bit float: 4 exponent bits, 3 mantissa bits, max 448  */
+} rns_kv_format;
+
+/*
+ * A cache of `pages` pages and the sequences that a call works on.  A page holds
+ * `page_tokens` tokens of every head; the page of one head is a block with one scale.
+ *   d_k, d_v              8-bit [pages, kv_heads, page_tokens, head_dim], 16-byte aligned
+ *   d_k_scale, d_v_scale  float [pages, kv_heads]
+ *   d_page_table          int32 [sequences, table_pages], row stride table_stride: page of
+ *                         tokens [i * page_tokens, (i+1) * page_tokens) of a sequence.  Entries
+ *                         beyond a sequence's length are not read.
+ *   d_status              int32 [1] or NULL
+ * page_tokens: 16, 32, 64 or 128; head_dim: a multiple of 16 up to 256.
+ *
+ * Lengths, starts and page indices are read on the device.  One that is out of range sets
+ * *d_status = RNS_ERR_BAD_INDEX and touches no memory: a sequence with a bad length or start
+ * counts as empty, a bad page is not written and reads as zeros.
+ * Sequences may share pages that are only read; a page that is written must belong to one
+ * sequence of the call.
+ */
+typedef struct rns_kv_cache {
+    int8_t* d_k;
+    int8_t* d_v;
+    float* d_k_scale;
+    float* d_v_scale;
+    int64_t pages;
+    int32_t page_tokens, kv_heads, head_dim;
+    int32_t format;
+    const int32_t* d_page_table;
+    int64_t table_stride;
+    int32_t table_pages, sequences;
+    int32_t* d_status;
+} rns_kv_cache;
+
+/*
+ * Host evaluation of the addressing the kernels use (same source, compiled for the CPU): with
+ * every pointer a host pointer, row_offsets[t], t in [0, tokens), receives the byte offset in d_k
+ * / d_v of new token t's row of head 0, or -1 where it has none (a dropped token, a bad page or
+ * sequence, rows of no sequence).  Bad entries set *cache->d_status as on the device.
+ */
+RNS_API int rns_host_kv_rows(const rns_kv_cache* cache, const int32_t* seq_lens, const int32_t* query_starts,
+                             int64_t tokens, int64_t* row_offsets);
+
+/*
+ * Quantises new tokens into the cache.  Sequence b's new tokens are rows
+ * [d_query_starts[b], d_query_starts[b+1]) of d_k_new / d_v_new ([tokens, kv_heads, head_dim],
+ * strides in elements, unit inner stride) and take the last positions of its d_seq_lens[b]
+ * tokens (the length AFTER the write); a new token whose position would be negative is dropped.
+ * Per touched block, in fp32:
+ *   s = max(max |x|, eps) / Q, at least the old scale where the block holds earlier tokens;
+ *   earlier tokens become round(q * (s_old / s)), new ones round(x / s), ties to even, clamped;
+ * eps = 2^-23, Q = 127 (int8) or 448 (e4m3).  A block that is given an infinity or NaN gets the
+ * scale NaN.  max_new: no sequence of the call has more new tokens (one that does is flagged
+ * and not written).  Rows of a block beyond the sequence's length stay as they are.
+ */
+RNS_API int rns_kv_write(const rns_kv_cache* cache, const void* d_k_new, const void* d_v_new,
+                         rns_float_type type, int64_t tokens,
+                         int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t v_token_stride, int64_t v_head_stride,
+                         const int32_t* d_seq_lens, const int32_t* d_query_starts, int max_new,
+                         rns_stream_t stream);
+
+/*
+ * Reads tokens back: rows [d_row_starts[b], d_row_starts[b+1]) of d_k_out / d_v_out
+ * ([rows, kv_heads, head_dim] contiguous, 16-byte aligned) receive type(f32(byte) * scale) of
+ * sequence b's tokens from position d_first[b] on.  max_rows: no sequence has more rows.
+ * Rows behind the last sequence's stay as they are.
+ */
+RNS_API int rns_kv_read(const rns_kv_cache* cache, const int32_t* d_first, const int32_t* d_row_starts,
+                        int64_t rows, int max_rows, void* d_k_out, void* d_v_out, rns_float_type type,
+                        rns_stream_t stream);
+
+/*
+ * Attention of new query tokens over the cached sequences:
+ *   out[t, h] = sum_j softmax_j(softmax_scale * q[t, h] . k[j, g]) v[j, g],   g = h / (heads / kv_heads)
+ * over the tokens j that query t sees.  Sequence b's queries are rows [d_query_starts[b],
+ * d_query_starts[b+1]) of d_q and sit at the last positions of its d_seq_lens[b] tokens: query i
+ * of n has position p = length - n + i.  It sees j <= p when causal, every j otherwise, and only
+ * j > p - window when window > 0 (window needs causal).  A query that sees nothing (p < 0, more
+ * queries than tokens or an empty sequence, included) gets zeros.
+ *   d_q    [tokens, heads, head_dim] F16 or BF16, strides in elements, unit inner stride
+ *   d_out  [tokens, heads, head_dim] of q's type, likewise; rows of no sequence stay as they are
+ *   d_lse  float [tokens, heads] or NULL: log of the sum of exp of the scaled scores (-inf where
+ *          a query sees nothing)
+ * max_new: as rns_kv_write.  d_workspace: rns_kv_attention_workspace() bytes of scratch of the
+ * caller's stream, 16-byte aligned; nothing in it has to be initialised.
+ */
+typedef struct rns_kv_attention_args {
+    const void* d_q;
+    int32_t type;                        /* RNS_F16 or RNS_BF16 */
+    int32_t heads;
+    int64_t tokens;
+    int64_t q_token_stride, q_head_stride;
+    const int32_t* d_seq_lens;
+    const int32_t* d_query_starts;
+    int32_t max_new;
+    int32_t causal, window;
+    float softmax_scale;
+    void* d_out;
+    int64_t out_token_stride, out_head_stride;
+    float* d_lse;
+    void* d_workspace;
+    int64_t workspace_bytes;
+} rns_kv_attention_args;
+
+RNS_API int64_t rns_kv_attention_workspace(const rns_kv_cache* cache, const rns_kv_attention_args* args);
+RNS_API int rns_kv_attention(const rns_kv_cache* cache, const rns_kv_attention_args* args, rns_stream_t stream);
 
 #ifdef __cplusplus
 }

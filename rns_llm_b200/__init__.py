@@ -4,6 +4,7 @@ from .backends import (
     CudaRNSBackend,
     PreparedAdaptiveRNSWeight,
     PreparedRNSWeight,
+    QuantizedKVCache,
     RNSRequestBatchWorkspace,
     RNSWorkspace,
     cuda_extension_available,
@@ -19,6 +20,7 @@ __all__ = [
     "CudaRNSBackend",
     "PreparedRNSWeight",
     "PreparedAdaptiveRNSWeight",
+    "QuantizedKVCache",
     "RNSWorkspace",
     "RNSRequestBatchWorkspace",
     "cuda_extension_available",

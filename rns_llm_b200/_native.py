@@ -23,11 +23,13 @@ TC_MAX_CHANNELS = 8
 MAX_PEERS = 7
 
 # rns_status
-OK, ERR_INVALID_ARGUMENT, ERR_BAD_MODULI, ERR_UNSUPPORTED, ERR_OVERFLOW, ERR_CUDA, ERR_DEVICE_TIMEOUT = range(7)
+OK, ERR_INVALID_ARGUMENT, ERR_BAD_MODULI, ERR_UNSUPPORTED, ERR_OVERFLOW, ERR_CUDA, ERR_DEVICE_TIMEOUT, ERR_BAD_INDEX = range(8)
 # rns_int_type / rns_out_type / rns_float_type
 INT8, INT16, INT32 = 0, 1, 2
 OUT_INT64, OUT_INT32, OUT_F16, OUT_BF16, OUT_F32 = 0, 1, 2, 3, 4
 F16, BF16, F32 = 0, 1, 2
+# rns_kv_format
+KV_INT8, KV_E4M3 = 0, 1
 
 
 class LinearArgs(C.Structure):
@@ -71,6 +73,33 @@ class LinearArgs(C.Structure):
         ("w_channel_stride", C.c_int64),
         ("out_copies_multicast", C.c_int32),
         ("groups", C.c_int32),
+    ]
+
+
+class KVCacheArgs(C.Structure):
+    """struct rns_kv_cache."""
+
+    _fields_ = [
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_k_scale", C.c_void_p), ("d_v_scale", C.c_void_p),
+        ("pages", C.c_int64),
+        ("page_tokens", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("format", C.c_int32),
+        ("d_page_table", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_pages", C.c_int32), ("sequences", C.c_int32),
+        ("d_status", C.c_void_p),
+    ]
+
+
+class KVAttentionArgs(C.Structure):
+    """struct rns_kv_attention_args."""
+
+    _fields_ = [
+        ("d_q", C.c_void_p), ("type", C.c_int32), ("heads", C.c_int32), ("tokens", C.c_int64),
+        ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("d_seq_lens", C.c_void_p), ("d_query_starts", C.c_void_p),
+        ("max_new", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("softmax_scale", C.c_float),
+        ("d_out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("d_lse", C.c_void_p), ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -119,6 +148,12 @@ SIGNATURES: dict[str, tuple] = {
     "rns_linear_static": (C.c_int, [_VP, C.c_int, C.c_int, C.c_int, C.c_int64, _VP, C.c_int, _I32P, C.c_int, _VP, _VP,
                                     _VP, C.c_int64, C.c_int32, _VP, _VP]),
     "rns_quantize_weight": (C.c_int, [_VP, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int, _VP, _VP, _VP, _VP]),
+    "rns_host_kv_rows": (C.c_int, [C.POINTER(KVCacheArgs), _VP, _VP, C.c_int64, _VP]),
+    "rns_kv_write": (C.c_int, [C.POINTER(KVCacheArgs), _VP, _VP, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                               C.c_int64, _VP, _VP, C.c_int, _VP]),
+    "rns_kv_read": (C.c_int, [C.POINTER(KVCacheArgs), _VP, _VP, C.c_int64, C.c_int, _VP, _VP, C.c_int, _VP]),
+    "rns_kv_attention_workspace": (C.c_int64, [C.POINTER(KVCacheArgs), C.POINTER(KVAttentionArgs)]),
+    "rns_kv_attention": (C.c_int, [C.POINTER(KVCacheArgs), C.POINTER(KVAttentionArgs), _VP]),
 }
 
 
@@ -161,6 +196,7 @@ _EXCEPTIONS = {
     ERR_OVERFLOW: OverflowError,
     ERR_CUDA: RuntimeError,
     ERR_DEVICE_TIMEOUT: RuntimeError,
+    ERR_BAD_INDEX: RuntimeError,
 }
 
 

@@ -7,12 +7,14 @@ from .cuda_backend import (
     RNSWorkspace,
     cuda_extension_available,
 )
+from .kv_cache import QuantizedKVCache
 
 __all__ = [
     "AdaptiveMetadata",
     "CudaRNSBackend",
     "PreparedRNSWeight",
     "PreparedAdaptiveRNSWeight",
+    "QuantizedKVCache",
     "RNSWorkspace",
     "RNSRequestBatchWorkspace",
     "cuda_extension_available",

@@ -38,6 +38,7 @@ from ..moduli import (
     garner_pairwise_inverses,
     validate_moduli,
 )
+from .kv_cache import KVCacheOperators
 
 CanonicalKernelName = Literal["auto", "naive", "tiled", "tiled_safe"]
 CenteredKernelName = Literal["auto", "scalar", "dp4a", "dp4a_safe", "cublas", "tcgen05", "planes"]
@@ -211,7 +212,7 @@ class _DeviceState:
     histogram: torch.Tensor       # int64 [MAX_CHANNELS+1]: adaptive selections per channel count
 
 
-class CudaRNSBackend:
+class CudaRNSBackend(KVCacheOperators):
     """RNS backend over hand-written sm_100a kernels (one process per GPU)."""
 
     name = "cuda-rns-b200"
@@ -282,6 +283,10 @@ class CudaRNSBackend:
             if code == N.ERR_OVERFLOW:
                 state.status.zero_()
                 raise OverflowError("full moduli set cannot represent the activation bound")
+            if code == N.ERR_BAD_INDEX:
+                state.status.zero_()
+                raise RuntimeError("a page index, sequence length or start that a key/value cache call read on the "
+                                   "device was out of range")
             if code != N.OK:
                 where = [int(v) for v in state.wait_info.cpu().tolist()]
                 state.status.zero_()
