@@ -824,8 +824,8 @@ static EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
-static int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                    const uint64_t* strides_bytes, const uint32_t* box, int tile_k) {
+int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+             const uint64_t* strides_bytes, const uint32_t* box, int tile_k) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return fail(RNS_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable in this driver");
     cuuint64_t gdim[3];

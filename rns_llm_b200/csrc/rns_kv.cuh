@@ -28,6 +28,25 @@ struct KvView {
     int32_t* status;
 };
 
+// The queries of one attention call.
+struct KvQuery {
+    const void* q;
+    int type;                      // RNS_F16 or RNS_BF16
+    int heads, group;              // group: query heads that share a head of the cache
+    int64_t tokens, q_token_stride, q_head_stride;
+    const int32_t *lens, *starts;
+    int causal, window;
+    float scale_log2;              // softmax scale / ln 2
+    void* out;
+    int64_t out_token_stride, out_head_stride;
+    float* lse;
+};
+
+// rns_kv_decode_sm100.cu.  Serves the sequences with at most max_rows_tokens new tokens; max_new sizes the row tiles.
+int64_t kv_decode_workspace(const KvView& c, const KvQuery& a, int max_new);
+int kv_decode(const KvView& c, const KvQuery& a, int format, int max_new, int max_rows_tokens, void* workspace,
+              cudaStream_t st);
+
 // Checks everything the host can see; RNS_OK fills `view`.
 int make_kv_view(const rns_kv_cache* cache, KvView* view);
 

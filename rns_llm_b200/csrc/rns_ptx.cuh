@@ -9,6 +9,11 @@ namespace rns {
 
 constexpr long long kWaitLimitCycles = 4000000000ll;  // about 2 s of SM clock
 
+// Tensor map of bytes, rank 2 or 3, boxes of tile_k = 64 or 128 inner bytes with the swizzle of that
+// width (rns_gemm_sm100.cu).  Returns an rns_status.
+int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+             const uint32_t* box, int tile_k);
+
 // ---------------------------------------------------------------------------
 // PTX wrappers
 // ---------------------------------------------------------------------------
