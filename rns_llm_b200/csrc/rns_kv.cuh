@@ -42,6 +42,14 @@ struct KvQuery {
     float* lse;
 };
 
+// Streaming multiprocessors of the current device.
+int sm_count(int* out);
+
+// rns_kv_prompt_sm100.cu: sequences with at least min_rows_tokens new tokens, heads of up to 128.
+bool kv_prompt_supported(const KvView& c);
+int64_t kv_prompt_workspace(const KvView& c);
+int kv_prompt(const KvView& c, const KvQuery& a, int format, int min_rows_tokens, void* workspace, cudaStream_t st);
+
 // rns_kv_decode_sm100.cu.  Serves the sequences with at most max_rows_tokens new tokens; max_new sizes the row tiles.
 int64_t kv_decode_workspace(const KvView& c, const KvQuery& a, int max_new);
 int kv_decode(const KvView& c, const KvQuery& a, int format, int max_new, int max_rows_tokens, void* workspace,

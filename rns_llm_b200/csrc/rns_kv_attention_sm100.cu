@@ -35,6 +35,33 @@ static int check_attention(const rns_kv_cache* cache, const rns_kv_attention_arg
     return RNS_OK;
 }
 
+// Which kernel serves which sequences: tiles of the rows kernel hold up to 32 query rows (new tokens x
+// heads that share one of the cache), those of the prompt kernel 256.
+struct Routing {
+    bool rows, prompt;
+    int rows_most;                 // new tokens of a sequence that the rows kernel takes, at most
+    int64_t rows_bytes, prompt_bytes;
+};
+static int route(const KvView& c, const KvQuery& a, int max_new, Routing* r) {
+    r->rows = r->prompt = false;
+    r->rows_bytes = r->prompt_bytes = 0;
+    r->rows_most = INT32_MAX;
+    if (max_new > a.tokens) max_new = (int)a.tokens;
+    if (kv_prompt_supported(c) && (int64_t)max_new * a.group > 32) {
+        r->prompt = true;
+        r->rows_most = 32 / a.group;
+        // few sequences can be much shorter than the longest: the prompt kernel takes them all
+        r->rows = r->rows_most > 0 && a.tokens * 4 < (int64_t)c.sequences * max_new * 3;
+        if (!r->rows) r->rows_most = 0;
+    } else {
+        r->rows = true;
+    }
+    if (r->rows) r->rows_bytes = kv_decode_workspace(c, a, r->prompt ? r->rows_most : max_new);
+    if (r->prompt) r->prompt_bytes = kv_prompt_workspace(c);
+    if (r->rows_bytes < 0 || r->prompt_bytes < 0) return RNS_ERR_CUDA;
+    return RNS_OK;
+}
+
 }  // namespace rns
 
 using namespace rns;
@@ -42,18 +69,28 @@ using namespace rns;
 extern "C" int64_t rns_kv_attention_workspace(const rns_kv_cache* cache, const rns_kv_attention_args* args) {
     KvView c;
     KvQuery p;
+    Routing r;
     if (int rc = check_attention(cache, args, &c, &p)) return -rc;
     if (c.sequences == 0 || p.tokens == 0) return 0;
-    return kv_decode_workspace(c, p, args->max_new);
+    if (int rc = route(c, p, args->max_new, &r)) return -rc;
+    return r.rows_bytes > r.prompt_bytes ? r.rows_bytes : r.prompt_bytes;
 }
 
 extern "C" int rns_kv_attention(const rns_kv_cache* cache, const rns_kv_attention_args* a, rns_stream_t stream) {
     KvView c;
     KvQuery p;
+    Routing r;
     if (int rc = check_attention(cache, a, &c, &p)) return rc;
     if (c.sequences == 0 || p.tokens == 0) return RNS_OK;
+    if (int rc = route(c, p, a->max_new, &r)) return rc;
     if ((reinterpret_cast<uintptr_t>(a->d_workspace) & 15) || a->d_workspace == nullptr ||
-        a->workspace_bytes < rns_kv_attention_workspace(cache, a))
+        a->workspace_bytes < r.rows_bytes || a->workspace_bytes < r.prompt_bytes)
         return fail(RNS_ERR_INVALID_ARGUMENT, "the workspace is missing, misaligned or too small");
-    return kv_decode(c, p, cache->format, a->max_new, INT32_MAX, a->d_workspace, reinterpret_cast<cudaStream_t>(stream));
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    // the two may share the workspace: the second starts when the first has finished
+    if (r.prompt)
+        if (int rc = kv_prompt(c, p, cache->format, r.rows ? r.rows_most + 1 : 0, a->d_workspace, st)) return rc;
+    if (r.rows)
+        return kv_decode(c, p, cache->format, r.prompt ? r.rows_most : a->max_new, r.rows_most, a->d_workspace, st);
+    return RNS_OK;
 }

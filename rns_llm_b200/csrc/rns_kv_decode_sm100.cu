@@ -25,8 +25,8 @@
 //   of their own.
 // * The running maximum may lag by 2^8 (a value scale by 2^4): then weights exceed one but nothing
 //   is lost, and the accumulators are rescaled only when a vote finds a larger score.  The maximum of
-//   a row follows that row's scores alone, and units are powers of two: what a row gives does not
-//   depend on the rows beside it.
+//   a row follows that row's scores alone, and units are powers of two: but for weights below fp16's
+//   normal range, what a row gives does not depend on the rows beside it.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ De
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-static int sm_count(int* out) {
+int sm_count(int* out) {
     int dev = 0;
     RNS_CUDA_OK(cudaGetDevice(&dev));
     RNS_CUDA_OK(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));

@@ -1,0 +1,870 @@
+// Attention of many query rows per sequence over the paged 8-bit cache (prompts and chunks of them),
+// heads of up to 128.
+//
+// A CTA works on two tiles of 128 query rows of one head of the cache (tokens x the heads that share
+// it) and walks the keys in blocks of 128.  Per block and tile:
+//     S = Q K^T          tcgen05, both operands fp16 in shared memory, S fp32 in tensor memory
+//     P = 2^(S f - m) w  one thread per row: S from tensor memory, P back into its place as fp16
+//     O += P V           tcgen05, P from tensor memory, V fp16 in shared memory, O in tensor memory
+// The bound is the tensor pipe (4 * 128 * 128 * head_dim operations a block and tile), with the
+// exponentials (16 a clock and SM) close behind; bytes from memory hardly count, since a block serves
+// 256 rows.  The two tiles keep the pipe busy in turn: one is multiplied while the other is
+// exponentiated.
+//
+// * The tensor cores have no product of fp16 with 8-bit operands, so four warps turn each 8-bit tile,
+//   as TMA brought it, into an fp16 tile in the swizzled layout of an operand: exactly, in whatever
+//   order of four neighbouring dimensions costs least (Q is laid out to match, O is put right when it
+//   is stored).  The same tile layout - 64 dimensions x 128 keys - is K-major for the first product
+//   and MN-major for the second, so V needs no transposition.
+// * Numerics are those of the rows kernel: queries times a power of two per row, fp32 scores, softmax
+//   and sums, weights rounded to fp16 in units of a power of two near the largest value scale; the
+//   running maximum may lag by 2^8, so that O in tensor memory is rescaled only now and then.
+// * Work is cut as there: one axis of key blocks over all items, equal shares, pieces joined by a
+//   second kernel.
+//
+// Warps 0-3 and 4-7: softmax of a tile (and its queries and outputs); 8-11: conversion; 12: issues the
+// products; 13: copies; 14: scales of the pages.
+#include "rns_kv.cuh"
+#include "rns_ptx.cuh"
+
+namespace rns {
+
+constexpr int kPromptThreads = 512;
+constexpr int kBlock = 128;               // keys of a block
+constexpr int kTileRows = 128;
+constexpr float kNoScore = -1.7e38f;      // below every score: "nothing seen yet"
+constexpr float kScoreLag = 8.0f;
+constexpr int kScaleSlots = 4;
+
+struct PromptParams {
+    KvView c;
+    KvQuery a;
+    int head_tile, token_tile, head_tiles;
+    int min_rows_tokens;                  // sequences with fewer new tokens are left to the rows kernel
+    int box_rows;
+    float sign;                           // of the softmax scale, which is folded into the queries
+    float* partial;                       // [grid][2][256 * (DIM + 2)]
+    int32_t* meta;                        // [grid][8]
+};
+
+struct PromptItem {
+    int b, kv_head, pair;
+    int64_t begin;
+    int count, length;
+    int token0, head0;                    // first token of the pair inside the sequence, first head of its head tile
+    int low, key0, blocks;                // first key that any row sees, rounded down to a block
+    int from[2], to[2];                   // blocks that a tile needs
+};
+
+__device__ __forceinline__ bool prompt_sequence(const PromptParams& p, int b, PromptItem& it) {
+    const KvSpan s = kv_span(p.c, p.a.lens, p.a.starts, p.a.tokens, b);
+    it.b = b; it.begin = s.begin; it.count = s.count; it.length = s.length;
+    return s.count >= p.min_rows_tokens && s.count > 0;
+}
+__device__ __forceinline__ int prompt_pairs(const PromptParams& p, int count) {
+    return (count + 2 * p.token_tile - 1) / (2 * p.token_tile) * p.head_tiles;
+}
+__device__ __forceinline__ void prompt_range(const PromptParams& p, PromptItem& it) {
+    it.token0 = it.pair / p.head_tiles * 2 * p.token_tile;
+    it.head0 = it.pair % p.head_tiles * p.head_tile;
+    const int base = it.length - it.count;
+    int first[2], last[2], low = INT32_MAX, high = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int ta = it.token0 + i * p.token_tile, tb = min(ta + p.token_tile, it.count);
+        first[i] = p.a.window > 0 ? max(0, base + ta - p.a.window + 1) : 0;
+        last[i] = p.a.causal ? base + tb : it.length;
+        if (ta >= it.count || base + tb <= 0) last[i] = 0;
+        if (last[i] > first[i]) { low = min(low, first[i]); high = max(high, last[i]); }
+    }
+    it.low = low;
+    it.key0 = high > 0 ? low & ~(kBlock - 1) : 0;
+    it.blocks = high > 0 ? (high - it.key0 + kBlock - 1) / kBlock : 1;    // nothing to see: zeros to write
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool sees = last[i] > first[i];
+        it.from[i] = sees ? (first[i] - it.key0) / kBlock : 0;
+        it.to[i] = sees ? (last[i] - it.key0 + kBlock - 1) / kBlock : 0;
+    }
+}
+__device__ __forceinline__ int64_t prompt_head_blocks(const PromptParams& p, PromptItem it) {
+    int64_t n = 0;
+    const int pairs = prompt_pairs(p, it.count);
+    for (it.pair = 0; it.pair < pairs; it.pair += p.head_tiles) {
+        prompt_range(p, it);
+        n += (int64_t)it.blocks * p.head_tiles;
+    }
+    return n;
+}
+
+// What one CTA has to do: blocks [step, stop) of item after item, `left` blocks in all.
+struct PromptWalk {
+    PromptItem it;
+    int step, stop;
+    int64_t left;
+
+    __device__ __forceinline__ void start(const PromptItem& first, int64_t rest, int64_t n) {
+        it = first; step = (int)rest; left = n;
+        stop = (int)min((int64_t)it.blocks, step + left);
+    }
+    // The next item's part; false at the end.
+    __device__ __forceinline__ bool next(const PromptParams& p) {
+        left -= stop - step;
+        if (left <= 0) return false;
+        if (++it.pair >= prompt_pairs(p, it.count)) {
+            it.pair = 0;
+            if (++it.kv_head >= p.c.kv_heads) {
+                it.kv_head = 0;
+                int b = it.b + 1;
+                while (b < p.c.sequences && !prompt_sequence(p, b, it)) ++b;
+                if (b >= p.c.sequences) return false;
+            }
+        }
+        prompt_range(p, it);
+        step = 0;
+        stop = (int)min((int64_t)it.blocks, left);
+        return true;
+    }
+    __device__ __forceinline__ bool active(int tile, int j) const { return j >= it.from[tile] && j < it.to[tile]; }
+    __device__ __forceinline__ bool live(int j) const { return active(0, j) || active(1, j); }
+    // blocks of this part that the tile needs
+    __device__ __forceinline__ int first_of(int tile) const { return max(step, it.from[tile]); }
+    __device__ __forceinline__ int end_of(int tile) const { return min(stop, it.to[tile]); }
+};
+
+template <int DIM> struct PromptShape {
+    static constexpr int kParts = DIM / 64;                        // 64-dimension parts of a tile
+    static constexpr int kTile = kBlock * DIM * 2;                 // fp16 tile of keys or values
+    static constexpr int kRaw = kBlock * DIM;                      // the same in 8 bits
+    static constexpr int kRing = 4, kRawRing = DIM == 64 ? 4 : 2;
+    static constexpr int kQ = 2 * kTileRows * DIM * 2;
+    static constexpr int kSmem = 1024 + kQ + kRing * kTile + kRawRing * kRaw;
+    static constexpr int kPartial = 2 * kTileRows * (DIM + 2);
+    static constexpr int kO = 256;                                 // tensor memory: S/P of the tiles at 0 and 128, O from here
+};
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ float prompt_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// fp16, K-major A; B K-major, or MN-major with `b_mn`.  fp32 accumulators.
+__device__ __forceinline__ constexpr uint32_t f16_idesc(uint32_t m, uint32_t n, bool b_mn) {
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// MN-major operand with 128-byte swizzle: 64 contiguous MN elements a row, rows along K 128 bytes
+// apart, groups of 8 rows `group` bytes apart, blocks of 64 MN elements `block` bytes apart.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr, uint32_t block, uint32_t group) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(group >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ uint32_t half_pair_s8(uint32_t x) {
+    uint32_t r = (x & 0x00ff00ffu) ^ 0x64806480u;                 // 1024 + 128 + value
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ uint32_t half_pair_e4m3(uint32_t x) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(x));
+    return r;
+}
+
+struct PromptBars {
+    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2], o_full[2], q_full[2];
+    uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
+};
+struct PromptScales {
+    float key[8], weight[8];              // of 16 keys each: key scale, value scale / unit
+    float unit, ratio;                    // this block's unit; the previous unit / this one
+    float pad[2];
+};
+
+template <int DIM, int FORMAT>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ PromptParams p) {
+    using S = PromptShape<DIM>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t q_smem = smem, ring = q_smem + S::kQ, raw = ring + S::kRing * S::kTile;
+    __shared__ PromptBars bars;
+    __shared__ __align__(16) PromptScales scales[kScaleSlots];
+    __shared__ int64_t scan[kPromptThreads / 32];
+    __shared__ PromptItem first_item;
+    __shared__ int64_t first_rest;
+    __shared__ int abort_word;
+    __shared__ uint32_t tmem_holder;
+
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    if (t == 0) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_addr(&bars.raw_full[i]), 1);
+            mbar_init(smem_addr(&bars.raw_empty[i]), 4);
+            mbar_init(smem_addr(&bars.full[i]), 4);
+            mbar_init(smem_addr(&bars.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&bars.s_full[i]), 1);
+            mbar_init(smem_addr(&bars.p_ready[i]), 4);
+            mbar_init(smem_addr(&bars.o_full[i]), 1);
+            mbar_init(smem_addr(&bars.q_full[i]), 4);
+        }
+        for (int i = 0; i < kScaleSlots; ++i) {
+            mbar_init(smem_addr(&bars.scale_full[i]), 1);
+            mbar_init(smem_addr(&bars.scale_empty[i]), 8);
+        }
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) { tmem_alloc(smem_addr(&tmem_holder), 512); tmem_relinquish(); }
+
+    // --- this CTA's share of the axis of key blocks
+    const int per = (p.c.sequences + kPromptThreads - 1) / kPromptThreads;
+    const int b0 = min(t * per, p.c.sequences), b1 = min(b0 + per, p.c.sequences);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        PromptItem it;
+        if (prompt_sequence(p, b, it)) mine += prompt_head_blocks(p, it) * p.c.kv_heads;
+    }
+    int64_t upto = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += v;
+    }
+    if (lane == 31) scan[warp] = upto;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_holder;
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kPromptThreads / 32; ++w) {
+        if (w < warp) upto += scan[w];
+        total += scan[w];
+    }
+    const int64_t ctas = min((int64_t)gridDim.x, total);
+    const int64_t w0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+    const int64_t w1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+    if (w0 < w1 && w0 >= upto - mine && w0 < upto) {               // exactly one thread
+        int64_t rest = w0 - (upto - mine);
+        PromptItem it;
+        for (int b = b0; b < b1; ++b) {
+            if (!prompt_sequence(p, b, it)) continue;
+            const int64_t per_head = prompt_head_blocks(p, it);
+            if (rest >= per_head * p.c.kv_heads) { rest -= per_head * p.c.kv_heads; continue; }
+            it.kv_head = (int)(rest / per_head);
+            rest -= it.kv_head * per_head;
+            for (it.pair = 0;; ++it.pair) {
+                prompt_range(p, it);
+                if (rest < it.blocks) break;
+                rest -= it.blocks;
+            }
+            break;
+        }
+        first_item = it;
+        first_rest = rest;
+    }
+    __syncthreads();
+    int32_t* meta = p.meta + (int64_t)blockIdx.x * 8;
+    if (t == 0) meta[0] = 0;
+
+    if (w0 < w1) {
+        PromptWalk walk;
+        walk.start(first_item, first_rest, w1 - w0);
+        volatile int* abort = &abort_word;
+
+        if (warp < 8) {
+            // ------------------------------------------------------------------ softmax
+            const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t s_tmem = tmem + tile * 128 + lanes, o_tmem = tmem + S::kO + tile * DIM + lanes;
+            const int row_token = row / p.head_tile, row_head = row - row_token * p.head_tile;
+            uint32_t s_uses = 0, o_uses = 0, scale_uses = 0;
+
+            // This row's query to shared memory as fp16 times a power of two; returns what the scores are times.
+            auto load_q = [&](const PromptItem& it) -> float {
+                const int tok = it.token0 + tile * p.token_tile + row_token, hd = it.head0 + row_head;
+                const bool there = row_token < p.token_tile && tok < it.count && hd < p.a.group;
+                const int64_t at = (it.begin + tok) * p.a.q_token_stride + ((int64_t)it.kv_head * p.a.group + hd) * p.a.q_head_stride;
+                const uint16_t* q = static_cast<const uint16_t*>(p.a.q) + at;
+                const bool vector = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+                uint32_t top = 0;
+                // two passes over the row (the second from L1): its largest magnitude, then the values
+#pragma unroll 1
+                for (int pass = 0; pass < 2; ++pass) {
+                    float up = 1.0f;
+                    if (pass == 1) {
+                        const int e = (int)(top >> 23);
+                        const int shift = top == 0 || e == 255 ? 0 : max(-126, min(120, 134 - e));
+                        up = __uint_as_float((uint32_t)(shift + 127) << 23) * p.sign;
+                        top = (uint32_t)(127 - max(-120, min(126, shift))) << 23;
+                    }
+#pragma unroll
+                    for (int c = 0; c < DIM / 8; ++c) {
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (there && c * 8 < p.c.head_dim) {
+                            if (vector) w = *reinterpret_cast<const uint4*>(q + c * 8);
+                            else {
+                                uint16_t e[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) e[i] = q[c * 8 + i];
+                                w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+                                               e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+                            }
+                        }
+                        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (p.a.type == RNS_F16) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&in[i]));
+                                v[2 * i] = f.x; v[2 * i + 1] = f.y;
+                            } else {
+                                v[2 * i] = __uint_as_float(in[i] << 16); v[2 * i + 1] = __uint_as_float(in[i] & 0xffff0000u);
+                            }
+                        }
+                        if (pass == 0) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(fabsf(v[i])));
+                        } else {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // int8 tiles hold dimensions 0 2 1 3 of every four
+                                const int a = FORMAT == RNS_KV_INT8 ? (i >> 1) * 4 + (i & 1) : 2 * i;
+                                const int b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1;
+                                const __half2 f = __floats2half2_rn(v[a] * up, v[b] * up);
+                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
+                            }
+                            const uint32_t to = q_smem + tile * (S::kQ / 2) + (c >> 3) * (kTileRows * 128) + row * 128 +
+                                                (((c & 7) ^ (row & 7)) << 4);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&bars.q_full[tile]));
+                return p.a.scale_log2 * p.sign * __uint_as_float(top);
+            };
+
+            float q_scale = walk.end_of(tile) > walk.first_of(tile) ? load_q(walk.it) : 0.0f;
+            bool ok = true, more = true;
+            while (more && ok) {
+                const PromptItem it = walk.it;
+                const int part_step = walk.step, part_stop = walk.stop;
+                const int64_t part_left = walk.left;
+                const int mine0 = walk.first_of(tile), mine1 = walk.end_of(tile);
+                const int tok = it.token0 + tile * p.token_tile + row_token;
+                const int position = it.length - it.count + tok;
+                const int hi = position < 0 ? 0 : p.a.causal ? position + 1 : it.length;
+                const int lo = p.a.window > 0 ? position - p.a.window + 1 : 0;
+                // keys that every row of the tile sees
+                const int tile_pos = it.length - it.count + it.token0 + tile * p.token_tile;
+                const int all_hi = p.a.causal ? tile_pos + 1 : tile_pos >= 0 ? it.length : 0;
+                const int all_lo = p.a.window > 0 ? tile_pos + p.token_tile - p.a.window : 0;
+                float m = kNoScore, l = 0.0f, unit = 0.0f;
+                for (int j = part_step; j < part_stop && ok; ++j) {
+                    if (!walk.live(j)) continue;
+                    const int slot = scale_uses % kScaleSlots;
+                    ok = warp_wait_bounded(smem_addr(&bars.scale_full[slot]), (scale_uses / kScaleSlots) & 1, abort, wait_code(1, slot));
+                    ++scale_uses;
+                    if (!ok) break;
+                    if (!walk.active(tile, j)) {
+                        if (lane == 0) mbar_arrive(smem_addr(&bars.scale_empty[slot]));
+                        continue;
+                    }
+                    ok = warp_wait_bounded(smem_addr(&bars.s_full[tile]), s_uses & 1, abort, wait_code(2, tile));
+                    ++s_uses;
+                    if (!ok) break;
+                    tc_fence_after();
+                    const PromptScales& sc = scales[slot];
+                    const int key = it.key0 + j * kBlock;
+                    const bool whole = key + kBlock <= all_hi && key >= all_lo;
+                    const int col_lo = lo - key, col_hi = hi - key;
+                    // pass 1: this row's largest score
+                    float top = kNoScore;
+#pragma unroll
+                    for (int ch = 0; ch < 4; ++ch) {
+                        float s[32];
+                        tmem_ld32(s_tmem + ch * 32, s);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            float best = -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int col = ch * 32 + g * 16 + i;
+                                const float v = whole || (col >= col_lo && col < col_hi) ? s[g * 16 + i] : -INFINITY;
+                                best = fmaxf(best, v);
+                            }
+                            top = fmaxf(top, best * (sc.key[ch * 2 + g] * q_scale));
+                        }
+                    }
+                    const bool first = j == mine0;
+                    if (!(top > m + kScoreLag)) top = m;
+                    const float keep = prompt_exp2(m - top), ratio = sc.ratio;
+                    m = top;
+                    unit = sc.unit;
+                    if (!first && __any_sync(0xffffffffu, keep != 1.0f || ratio != 1.0f)) {
+                        // S(j) has arrived, so the product of the block before has: O is at rest
+                        l *= keep;
+#pragma unroll
+                        for (int ch = 0; ch < DIM / 32; ++ch) {
+                            float o[32];
+                            tmem_ld32(o_tmem + ch * 32, o);
+                            tmem_ld_wait();
+                            uint32_t v[16];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[h * 16 + i] * (keep * ratio));
+                                tmem_st16(o_tmem + ch * 32 + h * 16, v);
+                            }
+                        }
+                    }
+                    // pass 2: weights
+#pragma unroll
+                    for (int ch = 0; ch < 4; ++ch) {
+                        float s[32];
+                        tmem_ld32(s_tmem + ch * 32, s);
+                        tmem_ld_wait();
+                        uint32_t w[16];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float f = sc.key[ch * 2 + g] * q_scale, weight = sc.weight[ch * 2 + g];
+                            float sum = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                float e0 = prompt_exp2(fmaf(s[g * 16 + i], f, -m)), e1 = prompt_exp2(fmaf(s[g * 16 + i + 1], f, -m));
+                                float p0 = e0 * weight, p1 = e1 * weight;
+                                if (!whole) {                       // not NaN from a scale that this row does not see
+                                    const int col = ch * 32 + g * 16 + i;
+                                    if (col < col_lo || col >= col_hi) e0 = p0 = 0.0f;
+                                    if (col + 1 < col_lo || col + 1 >= col_hi) e1 = p1 = 0.0f;
+                                }
+                                sum += e0 + e1;
+                                const __half2 h = __floats2half2_rn(p0, p1);
+                                w[g * 8 + i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            l += sum;
+                        }
+                        tmem_st16(s_tmem + ch * 16, w);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_addr(&bars.scale_empty[slot]));
+                        mbar_arrive(smem_addr(&bars.p_ready[tile]));
+                    }
+                }
+                if (!ok) break;
+                // the next part's queries before this one's output: their products can start meanwhile
+                more = walk.next(p);
+                const float next_scale = more && walk.end_of(tile) > walk.first_of(tile) ? load_q(walk.it) : 0.0f;
+                const bool any = mine1 > mine0;
+                if (any) {
+                    ok = warp_wait_bounded(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
+                    ++o_uses;
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                const bool begins = part_step == 0, ends = part_stop == it.blocks;
+                if (begins && ends) {
+                    const bool there = row_token < p.token_tile && tok < it.count && it.head0 + row_head < p.a.group;
+                    const int64_t token = it.begin + tok, head = (int64_t)it.kv_head * p.a.group + it.head0 + row_head;
+                    const bool empty = m == kNoScore && l == 0.0f;
+                    const float inv = empty ? 0.0f : unit / l;
+                    uint16_t* out = static_cast<uint16_t*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride;
+                    const bool vector = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+                    for (int ch = 0; ch < DIM / 32; ++ch) {
+                        float o[32];
+                        if (any) { tmem_ld32(o_tmem + ch * 32, o); tmem_ld_wait(); }
+                        uint32_t h[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int a = FORMAT == RNS_KV_INT8 ? (i >> 1) * 4 + (i & 1) : 2 * i;
+                            const int b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1;
+                            const float x = empty ? 0.0f : o[a] * inv, y = empty ? 0.0f : o[b] * inv;
+                            if (p.a.type == RNS_F16) {
+                                const __half2 f = __floats2half2_rn(x, y);
+                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
+                            } else {
+                                const __nv_bfloat162 f = __floats2bfloat162_rn(x, y);
+                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
+                            }
+                        }
+                        if (there) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (ch * 32 + i * 8 >= p.c.head_dim) break;
+                                if (vector) *reinterpret_cast<uint4*>(out + ch * 32 + i * 8) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                                else {
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) out[ch * 32 + i * 8 + e] = (uint16_t)(h[4 * i + e / 2] >> (16 * (e & 1)));
+                                }
+                            }
+                        }
+                    }
+                    if (p.a.lse != nullptr && there)
+                        p.a.lse[token * p.a.heads + head] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                } else {
+                    const int which = part_left == w1 - w0 ? 0 : 1;
+                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + which) * S::kPartial;
+                    const int at = tile * kTileRows + row;
+                    part[at] = m;
+                    part[2 * kTileRows + at] = l;
+                    float4* out = reinterpret_cast<float4*>(part + 4 * kTileRows + at * DIM);
+#pragma unroll
+                    for (int ch = 0; ch < DIM / 32; ++ch) {
+                        float o[32];
+                        if (any) { tmem_ld32(o_tmem + ch * 32, o); tmem_ld_wait(); }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int a = 4 * i, b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1, c = FORMAT == RNS_KV_INT8 ? a + 1 : a + 2;
+                            out[ch * 8 + i] = any ? make_float4(o[a] * unit, o[b] * unit, o[c] * unit, o[a + 3] * unit)
+                                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
+                    }
+                    if (begins && t == 0) {
+                        // this CTA holds the first piece: it names the item and where its pieces are
+                        const int64_t end = w1 - part_left + it.blocks;
+                        int64_t last = (end - 1) * ctas / total;
+                        while (total * (last + 1) / ctas < end) ++last;
+                        while (total * last / ctas > end - 1) --last;
+                        meta[1] = (int)(last - blockIdx.x) + 1;
+                        meta[2] = which;
+                        meta[3] = it.b; meta[4] = it.kv_head; meta[5] = it.token0; meta[6] = it.head0;
+                        meta[0] = 1;
+                    }
+                }
+                if (any) tc_fence_before();
+                q_scale = next_scale;
+            }
+        } else if (warp < 12) {
+            // ------------------------------------------------------------------ 8-bit tiles -> fp16 tiles
+            const int ct = t - 256;
+            uint32_t n = 0;
+            bool ok = true, more = true;
+            while (more && ok) {
+                for (int j = walk.step; j < walk.stop && ok; ++j) {
+                    if (!walk.live(j)) continue;
+                    const int valid = walk.it.length - (walk.it.key0 + j * kBlock);       // rows with a token
+                    for (int side = 0; side < 2; ++side, ++n) {
+                        const int rs = n % S::kRawRing, slot = n % S::kRing;
+                        ok = warp_wait_bounded(smem_addr(&bars.raw_full[rs]), (n / S::kRawRing) & 1, abort, wait_code(4, rs)) &&
+                             warp_wait_bounded(smem_addr(&bars.empty[slot]), ((n / S::kRing) & 1) ^ 1, abort, wait_code(5, slot));
+                        if (!ok) break;
+                        const uint32_t from = raw + rs * S::kRaw, to = ring + slot * S::kTile;
+                        constexpr int CHUNKS = DIM / 16;                                  // 16-byte chunks of a key
+#pragma unroll
+                        for (int i = 0; i < kBlock * CHUNKS / 128; ++i) {
+                            const int g = ct + i * 128, row = g / CHUNKS, c = g % CHUNKS;
+                            const uint32_t at = DIM == 64 ? from + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
+                                                          : from + row * 128 + ((c ^ (row & 7)) << 4);
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+                            // bytes behind the sequence may be NaN patterns, which no weight of zero removes
+                            if (FORMAT == RNS_KV_E4M3 && row >= valid) w[0] = w[1] = w[2] = w[3] = 0;
+                            uint32_t h[8];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if (FORMAT == RNS_KV_INT8) { h[2 * k] = half_pair_s8(w[k]); h[2 * k + 1] = half_pair_s8(w[k] >> 8); }
+                                else { h[2 * k] = half_pair_e4m3(w[k]); h[2 * k + 1] = half_pair_e4m3(w[k] >> 16); }
+                            }
+                            const uint32_t out = to + (c >> 2) * (kBlock * 128) + row * 128;
+                            const int c0 = 2 * (c & 3);
+                            // eight lanes hold one key of two parts: the upper part stores its second half first (banks)
+                            const bool swap = DIM == 128 && c >= 4;
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int half = swap ? 1 - k : k;
+                                const uint32_t dst = out + (((c0 + half) ^ (row & 7)) << 4);
+                                const uint32_t a0 = half ? h[4] : h[0], a1 = half ? h[5] : h[1], a2 = half ? h[6] : h[2], a3 = half ? h[7] : h[3];
+                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(a0), "r"(a1), "r"(a2), "r"(a3) : "memory");
+                            }
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(smem_addr(&bars.raw_empty[rs]));
+                            mbar_arrive(smem_addr(&bars.full[slot]));
+                        }
+                    }
+                }
+                more = ok && walk.next(p);
+            }
+        } else if (warp == 12) {
+            // ------------------------------------------------------------------ products
+            if (lane == 0) {
+                const uint32_t idesc_s = f16_idesc(128, kBlock, false), idesc_o = f16_idesc(128, DIM, true);
+                uint32_t n = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+                bool ok = true, more = true;
+                auto wait = [&](uint64_t& bar, uint32_t parity, int role, int index) {
+                    if (ok) ok = wait_bounded(smem_addr(&bar), parity & 1, abort, wait_code(role, index));
+                    tc_fence_after();
+                };
+                auto scores = [&](int tile, uint32_t slot) {
+#pragma unroll
+                    for (int k = 0; k < DIM / 16; ++k) {
+                        const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                        umma_f16(tmem + tile * 128, make_smem_desc(q_smem + tile * (S::kQ / 2) + off, 128),
+                                 make_smem_desc(ring + slot * S::kTile + off, 128), idesc_s, k > 0);
+                    }
+                    umma_commit(smem_addr(&bars.s_full[tile]));
+                };
+                while (more && ok) {
+                    int j = walk.step;
+                    while (j < walk.stop && !walk.live(j)) ++j;
+                    if (j < walk.stop) {
+                        for (int tile = 0; tile < 2 && ok; ++tile)
+                            if (walk.end_of(tile) > walk.first_of(tile)) wait(bars.q_full[tile], q_uses[tile]++, 6, tile);
+                        wait(bars.full[n % S::kRing], n / S::kRing, 7, n % S::kRing);
+                        if (!ok) break;
+                        for (int tile = 0; tile < 2; ++tile)
+                            if (walk.active(tile, j)) scores(tile, n % S::kRing);
+                        umma_commit(smem_addr(&bars.empty[n % S::kRing]));
+                        for (; j < walk.stop && walk.live(j) && ok; ++j, n += 2) {
+                            const uint32_t v = n + 1, k_next = n + 2;
+                            const bool again = j + 1 < walk.stop && walk.live(j + 1);
+                            wait(bars.full[v % S::kRing], v / S::kRing, 8, v % S::kRing);
+                            bool have = false;
+                            for (int tile = 0; tile < 2 && ok; ++tile) {
+                                if (walk.active(tile, j)) {
+                                    wait(bars.p_ready[tile], p_uses[tile]++, 9, tile);
+                                    if (!ok) break;
+                                    const bool first = j == walk.first_of(tile);
+#pragma unroll
+                                    for (int k = 0; k < kBlock / 16; ++k)
+                                        umma_f16_ts(tmem + S::kO + tile * DIM, tmem + tile * 128 + k * 8,
+                                                    mn_desc(ring + (v % S::kRing) * S::kTile + k * 2048, kBlock * 128, 1024),
+                                                    idesc_o, !(first && k == 0));
+                                    if (j + 1 == walk.end_of(tile)) umma_commit(smem_addr(&bars.o_full[tile]));
+                                }
+                                if (again && walk.active(tile, j + 1)) {
+                                    if (!have) wait(bars.full[k_next % S::kRing], k_next / S::kRing, 7, k_next % S::kRing);
+                                    have = true;
+                                    if (!ok) break;
+                                    scores(tile, k_next % S::kRing);
+                                }
+                            }
+                            if (!ok) break;
+                            umma_commit(smem_addr(&bars.empty[v % S::kRing]));
+                            if (again) umma_commit(smem_addr(&bars.empty[k_next % S::kRing]));
+                        }
+                    }
+                    more = ok && walk.next(p);
+                }
+                // nothing may still be on its way to this CTA's barriers when it leaves
+                for (uint32_t i = n > S::kRing ? n - S::kRing : 0; i < n && ok; ++i)
+                    wait(bars.empty[i % S::kRing], i / S::kRing, 10, i % S::kRing);
+            }
+            __syncwarp();
+        } else if (warp == 13) {
+            // ------------------------------------------------------------------ copies
+            uint32_t n = 0;
+            bool ok = true, more = true;
+            const int boxes = kBlock / p.box_rows;
+            while (more && ok) {
+                const PromptItem& it = walk.it;
+                for (int j = walk.step; j < walk.stop && ok; ++j) {
+                    if (!walk.live(j)) continue;
+                    const int key = it.key0 + j * kBlock + lane * p.box_rows;
+                    int z = (int)p.c.pages;                            // behind the last page: zeros
+                    if (lane < boxes && key < it.length) {
+                        const int page = kv_page(p.c, it.b, key >> p.c.page_shift);
+                        if (page >= 0) z = page;
+                    }
+                    for (int side = 0; side < 2; ++side, ++n) {
+                        const int rs = n % S::kRawRing;
+                        ok = warp_wait_bounded(smem_addr(&bars.raw_empty[rs]), ((n / S::kRawRing) & 1) ^ 1, abort, wait_code(11, rs));
+                        if (!ok) break;
+                        const uint32_t bar = smem_addr(&bars.raw_full[rs]);
+                        if (lane == 0) mbar_arrive_expect_tx(bar, S::kRaw);
+                        __syncwarp();
+                        if (lane < boxes)
+                            tma_load_3d(raw + rs * S::kRaw + lane * p.box_rows * DIM, side ? &map_v : &map_k, bar, 0,
+                                        it.kv_head * p.c.page_tokens + (key & (p.c.page_tokens - 1)), z);
+                    }
+                }
+                more = ok && walk.next(p);
+            }
+        } else if (warp == 14) {
+            // ------------------------------------------------------------------ scales of the pages
+            uint32_t n = 0;
+            bool ok = true, more = true;
+            while (more && ok) {
+                const PromptItem& it = walk.it;
+                float unit = 0x1p-123f;
+                for (int j = walk.step; j < walk.stop && ok; ++j) {
+                    if (!walk.live(j)) continue;
+                    const int key = it.key0 + j * kBlock + (lane & 7) * 16;
+                    float ks = 0.0f, vs = 0.0f;
+                    if (key < it.length) {
+                        const int page = kv_page(p.c, it.b, key >> p.c.page_shift);
+                        if (page >= 0) {
+                            const int64_t block = (int64_t)page * p.c.kv_heads + it.kv_head;
+                            ks = p.c.scale[0][block];
+                            vs = p.c.scale[1][block];
+                        }
+                    }
+                    if (!(fabsf(vs) <= 3.0e38f)) vs = __uint_as_float(0x7fc00000u);
+                    // the largest of the finite ones that some row sees
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, vs == vs && key + 16 > it.low ? __float_as_uint(fabsf(vs)) : 0u);
+                    float ratio = 1.0f;
+                    if (__uint_as_float(top) > 16.0f * unit) {
+                        const float grown = __uint_as_float(top & 0x7f800000u);
+                        ratio = unit / grown;
+                        unit = grown;
+                    }
+                    const int slot = n % kScaleSlots;
+                    ok = warp_wait_bounded(smem_addr(&bars.scale_empty[slot]), ((n / kScaleSlots) & 1) ^ 1, abort, wait_code(12, slot));
+                    if (!ok) break;
+                    ++n;
+                    if (lane < 8) { scales[slot].key[lane] = ks; scales[slot].weight[lane] = vs / unit; }
+                    if (lane == 0) { scales[slot].unit = unit; scales[slot].ratio = ratio; }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&bars.scale_full[slot]));
+                }
+                more = ok && walk.next(p);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (abort_word != 0 && t == 0 && p.c.status != nullptr) *p.c.status = RNS_ERR_DEVICE_TIMEOUT;
+}
+
+// Joins the pieces of the items that a CTA boundary cut: block (first piece's CTA, 8 rows), a warp a row.
+template <int DIM>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_constant__ PromptParams p) {
+    using S = PromptShape<DIM>;
+    asm volatile("griddepcontrol.wait;" ::: "memory");             // the pieces are complete and visible
+    const int32_t* meta = p.meta + (int64_t)blockIdx.x * 8;
+    if (meta[0] == 0) return;
+    const int lane = threadIdx.x & 31, at = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int tile = at / kTileRows, row = at % kTileRows;
+    const int row_token = row / p.head_tile, row_head = row - row_token * p.head_tile;
+    const KvSpan s = kv_span(p.c, p.a.lens, p.a.starts, p.a.tokens, meta[3]);
+    const int tok = meta[5] + tile * p.token_tile + row_token, hd = meta[6] + row_head;
+    if (row_token >= p.token_tile || tok >= s.count || hd >= p.a.group) return;
+    const int pieces = meta[1];
+    const float* first = p.partial + ((int64_t)blockIdx.x * 2 + meta[2]) * S::kPartial;
+    const float* next = p.partial + ((int64_t)blockIdx.x + 1) * 2 * S::kPartial;
+    float top = first[at];
+    for (int i = 1; i < pieces; ++i) top = fmaxf(top, next[(int64_t)(i - 1) * 2 * S::kPartial + at]);
+    float sum = 0.0f, o[DIM / 32] = {};
+    for (int i = 0; i < pieces; ++i) {
+        const float* part = i == 0 ? first : next + (int64_t)(i - 1) * 2 * S::kPartial;
+        const float f = prompt_exp2(part[at] - top);
+        sum = fmaf(part[2 * kTileRows + at], f, sum);
+#pragma unroll
+        for (int j = 0; j < DIM / 32; ++j) o[j] = fmaf(part[4 * kTileRows + at * DIM + j * 32 + lane], f, o[j]);
+    }
+    const bool empty = top == kNoScore && sum == 0.0f;
+    const float inv = empty ? 0.0f : 1.0f / sum;
+    const int64_t token = s.begin + tok, head = (int64_t)meta[4] * p.a.group + hd;
+#pragma unroll
+    for (int j = 0; j < DIM / 32; ++j) {
+        const int d = j * 32 + lane;
+        if (d >= p.c.head_dim) continue;
+        const int64_t to = token * p.a.out_token_stride + head * p.a.out_head_stride + d;
+        if (p.a.type == RNS_F16) static_cast<__half*>(p.a.out)[to] = __float2half_rn(o[j] * inv);
+        else static_cast<__nv_bfloat16*>(p.a.out)[to] = __float2bfloat16_rn(o[j] * inv);
+    }
+    if (p.a.lse != nullptr && lane == 0)
+        p.a.lse[token * p.a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+bool kv_prompt_supported(const KvView& c) { return c.head_dim <= 128; }
+
+int64_t kv_prompt_workspace(const KvView& c) {
+    int sms = 0;
+    if (sm_count(&sms) != RNS_OK) return -RNS_ERR_CUDA;
+    return (int64_t)sms * (2 * (c.head_dim <= 64 ? PromptShape<64>::kPartial : PromptShape<128>::kPartial) * 4 + 32);
+}
+
+template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* workspace, cudaStream_t st) {
+    using S = PromptShape<DIM>;
+    static_assert(S::kSmem + 2048 <= 227 * 1024, "one CTA per SM");
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    p.box_rows = p.c.page_tokens;
+    CUtensorMap maps[2];
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t dims[3] = {(uint64_t)p.c.head_dim, (uint64_t)p.c.kv_heads * p.c.page_tokens, (uint64_t)p.c.pages};
+        const uint64_t strides[2] = {dims[0], dims[0] * dims[1]};
+        const uint32_t box[3] = {(uint32_t)DIM, (uint32_t)p.box_rows, 1u};
+        if (int rc = make_map(&maps[i], p.c.data[i], 3, dims, strides, box, DIM)) return rc;
+    }
+    p.meta = static_cast<int32_t*>(workspace);
+    p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)sms * 32);
+    const auto kernel = kv_prompt_kernel<DIM, FORMAT>;
+    RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    kernel<<<sms, kPromptThreads, S::kSmem, st>>>(maps[0], maps[1], p);
+    RNS_CUDA_OK(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)sms, 2 * kTileRows / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    RNS_CUDA_OK(cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<DIM>, p));
+    return RNS_OK;
+}
+
+int kv_prompt(const KvView& c, const KvQuery& a, int format, int min_rows_tokens, void* workspace, cudaStream_t st) {
+    PromptParams p;
+    memset(&p, 0, sizeof(p));
+    p.c = c; p.a = a;
+    p.min_rows_tokens = min_rows_tokens;
+    p.sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+    p.head_tile = a.group < kTileRows ? a.group : kTileRows;
+    p.token_tile = kTileRows / p.head_tile;
+    p.head_tiles = (a.group + p.head_tile - 1) / p.head_tile;
+    if (c.head_dim <= 64)
+        return format == RNS_KV_INT8 ? launch_prompt<64, RNS_KV_INT8>(p, workspace, st) : launch_prompt<64, RNS_KV_E4M3>(p, workspace, st);
+    return format == RNS_KV_INT8 ? launch_prompt<128, RNS_KV_INT8>(p, workspace, st) : launch_prompt<128, RNS_KV_E4M3>(p, workspace, st);
+}
+
+}  // namespace rns

@@ -3,8 +3,10 @@
 Writing and reading are compared bit for bit (both sides are correctly rounded fp32).  Attention is
 compared with float64 element by element; the bound counts, per output,
 * half a step of the output type,
-* the rounding of each softmax weight to fp16 before it meets the values, 2^-11 of sum p|v| (weights
-  below fp16's normal range add at most 2^-25 of the largest value of any page each),
+* the rounding of each softmax weight to fp16 before it meets the values, 2^-11 of sum p|v|.  A weight
+  below fp16's normal range, 2^-14, is off by up to half of its step 2^-24, in units of a value scale that
+  is at most the largest of the pages: times the byte it meets that is 2^-25 of the largest value, for
+  each of the `keys` weights; the sum they are divided by is at least 1 (the maximum's own weight);
 * scores in fp32: head_dim + 8 roundings of 2^-22 (tensor cores truncate) of sum |q k|, which move a
   weight by that relative amount, twice (numerator and denominator), and so the output by that of
   sum p|v|;
@@ -215,7 +217,7 @@ def test_read_is_bit_exact(backend, lens, first, heads, dim, page, fmt, dtype):
 def attention_bound(want, spread, loud, dim, dtype, keys, largest):
     score = (dim + 8) * 2.0 ** -22 * loud[:, :, None]
     return (HALF_STEP[dtype] * np.abs(want) + (2.0 ** -11 + 2.0 ** -20 + 2 * score) * spread * 1.01 +
-            keys * 2.0 ** -25 * largest / max(keys, 1) + 2.0 ** -24)
+            keys * 2.0 ** -25 * largest + 2.0 ** -24)
 
 
 def check_attention(s, q, new, got, lse, *, scale, causal=True, window=0, dtype):
