@@ -23,7 +23,7 @@
 //   second kernel.
 //
 // Warps 0-3 and 4-7: softmax of a tile (and its queries and outputs); 8-11: conversion; 12: issues the
-// products; 13: copies; 14: scales of the pages.
+// products; 13: copies; 14: scales of the pages; 15: the list of what there is to do.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 
@@ -34,7 +34,7 @@ constexpr int kBlock = 128;               // keys of a block
 constexpr int kTileRows = 128;
 constexpr float kNoScore = -1.7e38f;      // below every score: "nothing seen yet"
 constexpr float kScoreLag = 8.0f;
-constexpr int kScaleSlots = 4;
+constexpr int kScaleSlots = 4, kPartSlots = 4;
 
 struct PromptParams {
     KvView c;
@@ -97,40 +97,44 @@ __device__ __forceinline__ int64_t prompt_head_blocks(const PromptParams& p, Pro
     return n;
 }
 
-// What one CTA has to do: blocks [step, stop) of item after item, `left` blocks in all.
-struct PromptWalk {
+// What a CTA does is a list of parts: blocks [step, stop) of item after item.  One warp walks the
+// axis and publishes the parts; the others read them from shared memory.
+struct PromptPart {
     PromptItem it;
     int step, stop;
-    int64_t left;
+    int live0, live1;                     // blocks of the part that some tile needs (one range: the tiles' meet)
+    int mine0[2], mine1[2];               // blocks of it that each tile needs
+    int64_t left;                         // blocks of the CTA from this part on
+    int last;                             // no part follows
 
-    __device__ __forceinline__ void start(const PromptItem& first, int64_t rest, int64_t n) {
-        it = first; step = (int)rest; left = n;
+    __device__ __forceinline__ void set(int from, int64_t blocks) {
+        step = from; left = blocks;
         stop = (int)min((int64_t)it.blocks, step + left);
-    }
-    // The next item's part; false at the end.
-    __device__ __forceinline__ bool next(const PromptParams& p) {
-        left -= stop - step;
-        if (left <= 0) return false;
-        if (++it.pair >= prompt_pairs(p, it.count)) {
-            it.pair = 0;
-            if (++it.kv_head >= p.c.kv_heads) {
-                it.kv_head = 0;
-                int b = it.b + 1;
-                while (b < p.c.sequences && !prompt_sequence(p, b, it)) ++b;
-                if (b >= p.c.sequences) return false;
-            }
+        live0 = INT32_MAX; live1 = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mine0[i] = max(step, it.from[i]);
+            mine1[i] = min(stop, it.to[i]);
+            if (mine1[i] > mine0[i]) { live0 = min(live0, mine0[i]); live1 = max(live1, mine1[i]); }
+            else mine0[i] = mine1[i] = 0;
         }
-        prompt_range(p, it);
-        step = 0;
-        stop = (int)min((int64_t)it.blocks, left);
-        return true;
+        if (live1 == 0) live0 = 0;
+        last = left <= stop - step;
     }
-    __device__ __forceinline__ bool active(int tile, int j) const { return j >= it.from[tile] && j < it.to[tile]; }
-    __device__ __forceinline__ bool live(int j) const { return active(0, j) || active(1, j); }
-    // blocks of this part that the tile needs
-    __device__ __forceinline__ int first_of(int tile) const { return max(step, it.from[tile]); }
-    __device__ __forceinline__ int end_of(int tile) const { return min(stop, it.to[tile]); }
 };
+__device__ __forceinline__ void prompt_next(const PromptParams& p, PromptPart& part) {
+    PromptItem& it = part.it;
+    if (++it.pair >= prompt_pairs(p, it.count)) {
+        it.pair = 0;
+        if (++it.kv_head >= p.c.kv_heads) {
+            it.kv_head = 0;
+            int b = it.b + 1;
+            while (b < p.c.sequences && !prompt_sequence(p, b, it)) ++b;
+        }
+    }
+    prompt_range(p, it);
+    part.set(0, part.left - (part.stop - part.step));
+}
 
 template <int DIM> struct PromptShape {
     static constexpr int kParts = DIM / 64;                        // 64-dimension parts of a tile
@@ -155,17 +159,51 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t* u = reinterpret_cast<uint32_t*>(v);
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
-          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
-          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 __device__ __forceinline__ float prompt_exp2(float x) {
     float r;
@@ -198,15 +236,70 @@ __device__ __forceinline__ uint32_t half_pair_e4m3(uint32_t x) {
     return r;
 }
 
+// Waits of whole warps.  Sixteen warps run eight different programs here, and the instruction cache is
+// what they compete for first (inlined waits and fully unrolled rows of 128 columns made "no
+// instruction" the largest stall by far): the waiting itself is one function for all of them.
+__device__ __noinline__ bool prompt_wait_long(uint32_t bar, uint32_t parity, volatile int* abort, int where) {
+    const long long t0 = clock64();
+    for (uint32_t spin = 1;; ++spin) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((spin & 255u) == 0) {
+            if (*abort) return false;
+            if (clock64() - t0 > kWaitLimitCycles) {
+                if (*abort == 0) *abort = where;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity, volatile int* abort, int where) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (!__all_sync(0xffffffffu, ok)) {
+        if (!ok) ok = prompt_wait_long(bar, parity, abort, where);
+        ok = __all_sync(0xffffffffu, ok);
+    }
+    return ok;
+}
+
 struct PromptBars {
     uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2], o_full[2], q_full[2];
-    uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
+    uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots], part_full[kPartSlots], part_empty[kPartSlots];
 };
 struct PromptScales {
     float key[8], weight[8];              // of 16 keys each: key scale, value scale / unit
     float unit, ratio;                    // this block's unit; the previous unit / this one
     float pad[2];
 };
+
+// 32 of a row's scores -> weights 2^(s f - m), added up in `sum`, and times the values' scale as fp16 to
+// tensor memory.  WHOLE: the row sees every column; otherwise the bits of `seen` say which.
+template <bool WHOLE>
+__device__ __forceinline__ void prompt_weights(const float (&s)[32], uint32_t seen, const float* key, const float* weights,
+                                               float q_scale, float m, uint32_t tmem, float2& sum) {
+    const float2 minus_m = make_float2(-m, -m);
+    uint32_t w[16];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const float f = key[g] * q_scale, weight = weights[g];
+        float2 e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = fma2(make_float2(s[g * 16 + 2 * i], s[g * 16 + 2 * i + 1]), make_float2(f, f), minus_m);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = make_float2(prompt_exp2(e[i].x), prompt_exp2(e[i].y));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float2 pw = mul2(e[i], make_float2(weight, weight));
+            if (!WHOLE) {                                           // not NaN from a scale that this row does not see
+                if (!((seen >> (g * 16 + 2 * i)) & 1)) e[i].x = pw.x = 0.0f;
+                if (!((seen >> (g * 16 + 2 * i + 1)) & 1)) e[i].y = pw.y = 0.0f;
+            }
+            sum = add2(sum, e[i]);
+            const __half2 h = __floats2half2_rn(pw.x, pw.y);
+            w[g * 8 + i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    tmem_st16(tmem, w);
+}
 
 template <int DIM, int FORMAT>
 __global__ void __launch_bounds__(kPromptThreads, 1)
@@ -219,8 +312,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __shared__ PromptBars bars;
     __shared__ __align__(16) PromptScales scales[kScaleSlots];
     __shared__ int64_t scan[kPromptThreads / 32];
-    __shared__ PromptItem first_item;
-    __shared__ int64_t first_rest;
+    __shared__ PromptPart parts[kPartSlots];
     __shared__ int abort_word;
     __shared__ uint32_t tmem_holder;
 
@@ -241,6 +333,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         for (int i = 0; i < kScaleSlots; ++i) {
             mbar_init(smem_addr(&bars.scale_full[i]), 1);
             mbar_init(smem_addr(&bars.scale_empty[i]), 8);
+        }
+        for (int i = 0; i < kPartSlots; ++i) {
+            mbar_init(smem_addr(&bars.part_full[i]), 1);
+            mbar_init(smem_addr(&bars.part_empty[i]), 15);         // every warp but the one that writes them
         }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -291,17 +387,26 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             }
             break;
         }
-        first_item = it;
-        first_rest = rest;
+        parts[0].it = it;
+        parts[0].set((int)rest, w1 - w0);
     }
     __syncthreads();
     int32_t* meta = p.meta + (int64_t)blockIdx.x * 8;
     if (t == 0) meta[0] = 0;
 
     if (w0 < w1) {
-        PromptWalk walk;
-        walk.start(first_item, first_rest, w1 - w0);
         volatile int* abort = &abort_word;
+        uint32_t n_part = 0;
+        // The next part of the list (the first is there from the start), and giving its slot back.
+        auto part_wait = [&]() -> bool {
+            return n_part == 0 || prompt_wait(smem_addr(&bars.part_full[n_part % kPartSlots]),
+                                                    (n_part / kPartSlots) & 1, abort, wait_code(13, n_part % kPartSlots));
+        };
+        auto part_done = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&bars.part_empty[n_part % kPartSlots]));
+            ++n_part;
+        };
 
         if (warp < 8) {
             // ------------------------------------------------------------------ softmax
@@ -378,13 +483,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 return p.a.scale_log2 * p.sign * __uint_as_float(top);
             };
 
-            float q_scale = walk.end_of(tile) > walk.first_of(tile) ? load_q(walk.it) : 0.0f;
+            float q_scale = parts[0].mine1[tile] > parts[0].mine0[tile] ? load_q(parts[0].it) : 0.0f;
             bool ok = true, more = true;
             while (more && ok) {
-                const PromptItem it = walk.it;
-                const int part_step = walk.step, part_stop = walk.stop;
-                const int64_t part_left = walk.left;
-                const int mine0 = walk.first_of(tile), mine1 = walk.end_of(tile);
+                const PromptPart& part = parts[n_part % kPartSlots];
+                const PromptItem& it = part.it;
+                const int mine0 = part.mine0[tile], mine1 = part.mine1[tile], live1 = part.live1, key0 = it.key0;
                 const int tok = it.token0 + tile * p.token_tile + row_token;
                 const int position = it.length - it.count + tok;
                 const int hi = position < 0 ? 0 : p.a.causal ? position + 1 : it.length;
@@ -394,40 +498,46 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int all_hi = p.a.causal ? tile_pos + 1 : tile_pos >= 0 ? it.length : 0;
                 const int all_lo = p.a.window > 0 ? tile_pos + p.token_tile - p.a.window : 0;
                 float m = kNoScore, l = 0.0f, unit = 0.0f;
-                for (int j = part_step; j < part_stop && ok; ++j) {
-                    if (!walk.live(j)) continue;
+                for (int j = part.live0; j < live1; ++j) {
                     const int slot = scale_uses % kScaleSlots;
-                    ok = warp_wait_bounded(smem_addr(&bars.scale_full[slot]), (scale_uses / kScaleSlots) & 1, abort, wait_code(1, slot));
+                    ok = prompt_wait(smem_addr(&bars.scale_full[slot]), (scale_uses / kScaleSlots) & 1, abort, wait_code(1, slot));
                     ++scale_uses;
                     if (!ok) break;
-                    if (!walk.active(tile, j)) {
+                    if (j < mine0 || j >= mine1) {
                         if (lane == 0) mbar_arrive(smem_addr(&bars.scale_empty[slot]));
                         continue;
                     }
-                    ok = warp_wait_bounded(smem_addr(&bars.s_full[tile]), s_uses & 1, abort, wait_code(2, tile));
+                    ok = prompt_wait(smem_addr(&bars.s_full[tile]), s_uses & 1, abort, wait_code(2, tile));
                     ++s_uses;
                     if (!ok) break;
                     tc_fence_after();
                     const PromptScales& sc = scales[slot];
-                    const int key = it.key0 + j * kBlock;
+                    const int key = key0 + j * kBlock;
                     const bool whole = key + kBlock <= all_hi && key >= all_lo;
                     const int col_lo = lo - key, col_hi = hi - key;
-                    // pass 1: this row's largest score
+                    // bits [col_lo, col_hi) of a chunk's 32 columns: those this row sees
+                    const auto seen = [&](int ch) {
+                        const int a = min(max(col_lo - ch * 32, 0), 32), b = min(max(col_hi - ch * 32, 0), 32);
+                        return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
+                    };
+                    // this row's largest score
                     float top = kNoScore;
-#pragma unroll
+#pragma unroll 1
                     for (int ch = 0; ch < 4; ++ch) {
                         float s[32];
                         tmem_ld32(s_tmem + ch * 32, s);
                         tmem_ld_wait();
+                        if (!whole) {
+                            const uint32_t bits = seen(ch);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!((bits >> i) & 1)) s[i] = -INFINITY;
+                        }
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            float best = -INFINITY;
+                            float best = s[g * 16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int col = ch * 32 + g * 16 + i;
-                                const float v = whole || (col >= col_lo && col < col_hi) ? s[g * 16 + i] : -INFINITY;
-                                best = fmaxf(best, v);
-                            }
+                            for (int i = 1; i < 16; ++i) best = fmaxf(best, s[g * 16 + i]);
                             top = fmaxf(top, best * (sc.key[ch * 2 + g] * q_scale));
                         }
                     }
@@ -439,48 +549,28 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     if (!first && __any_sync(0xffffffffu, keep != 1.0f || ratio != 1.0f)) {
                         // S(j) has arrived, so the product of the block before has: O is at rest
                         l *= keep;
-#pragma unroll
-                        for (int ch = 0; ch < DIM / 32; ++ch) {
-                            float o[32];
-                            tmem_ld32(o_tmem + ch * 32, o);
-                            tmem_ld_wait();
+#pragma unroll 1
+                        for (int ch = 0; ch < DIM / 16; ++ch) {
+                            float o[16];
                             uint32_t v[16];
+                            tmem_ld16(o_tmem + ch * 16, o);
+                            tmem_ld_wait();
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[h * 16 + i] * (keep * ratio));
-                                tmem_st16(o_tmem + ch * 32 + h * 16, v);
-                            }
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[i] * (keep * ratio));
+                            tmem_st16(o_tmem + ch * 16, v);
                         }
                     }
-                    // pass 2: weights
-#pragma unroll
+                    // weights, in place of the scores
+                    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
                     for (int ch = 0; ch < 4; ++ch) {
                         float s[32];
                         tmem_ld32(s_tmem + ch * 32, s);
                         tmem_ld_wait();
-                        uint32_t w[16];
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const float f = sc.key[ch * 2 + g] * q_scale, weight = sc.weight[ch * 2 + g];
-                            float sum = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                float e0 = prompt_exp2(fmaf(s[g * 16 + i], f, -m)), e1 = prompt_exp2(fmaf(s[g * 16 + i + 1], f, -m));
-                                float p0 = e0 * weight, p1 = e1 * weight;
-                                if (!whole) {                       // not NaN from a scale that this row does not see
-                                    const int col = ch * 32 + g * 16 + i;
-                                    if (col < col_lo || col >= col_hi) e0 = p0 = 0.0f;
-                                    if (col + 1 < col_lo || col + 1 >= col_hi) e1 = p1 = 0.0f;
-                                }
-                                sum += e0 + e1;
-                                const __half2 h = __floats2half2_rn(p0, p1);
-                                w[g * 8 + i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
-                            l += sum;
-                        }
-                        tmem_st16(s_tmem + ch * 16, w);
+                        if (whole) prompt_weights<true>(s, 0, &sc.key[ch * 2], &sc.weight[ch * 2], q_scale, m, s_tmem + ch * 16, sum);
+                        else prompt_weights<false>(s, seen(ch), &sc.key[ch * 2], &sc.weight[ch * 2], q_scale, m, s_tmem + ch * 16, sum);
                     }
+                    l += sum.x + sum.y;
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -491,16 +581,24 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 if (!ok) break;
                 // the next part's queries before this one's output: their products can start meanwhile
-                more = walk.next(p);
-                const float next_scale = more && walk.end_of(tile) > walk.first_of(tile) ? load_q(walk.it) : 0.0f;
+                more = !part.last;
+                float next_scale = 0.0f;
+                if (more) {
+                    ++n_part;
+                    ok = part_wait();
+                    const PromptPart& next = parts[n_part % kPartSlots];
+                    if (ok && next.mine1[tile] > next.mine0[tile]) next_scale = load_q(next.it);
+                    --n_part;
+                    if (!ok) break;
+                }
                 const bool any = mine1 > mine0;
                 if (any) {
-                    ok = warp_wait_bounded(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
+                    ok = prompt_wait(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
                     ++o_uses;
                     if (!ok) break;
                     tc_fence_after();
                 }
-                const bool begins = part_step == 0, ends = part_stop == it.blocks;
+                const bool begins = part.step == 0, ends = part.stop == it.blocks;
                 if (begins && ends) {
                     const bool there = row_token < p.token_tile && tok < it.count && it.head0 + row_head < p.a.group;
                     const int64_t token = it.begin + tok, head = (int64_t)it.kv_head * p.a.group + it.head0 + row_head;
@@ -541,12 +639,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     if (p.a.lse != nullptr && there)
                         p.a.lse[token * p.a.heads + head] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                 } else {
-                    const int which = part_left == w1 - w0 ? 0 : 1;
-                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + which) * S::kPartial;
+                    const int which = part.left == w1 - w0 ? 0 : 1;
+                    float* piece = p.partial + ((int64_t)blockIdx.x * 2 + which) * S::kPartial;
                     const int at = tile * kTileRows + row;
-                    part[at] = m;
-                    part[2 * kTileRows + at] = l;
-                    float4* out = reinterpret_cast<float4*>(part + 4 * kTileRows + at * DIM);
+                    piece[at] = m;
+                    piece[2 * kTileRows + at] = l;
+                    float4* out = reinterpret_cast<float4*>(piece + 4 * kTileRows + at * DIM);
 #pragma unroll
                     for (int ch = 0; ch < DIM / 32; ++ch) {
                         float o[32];
@@ -560,7 +658,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     }
                     if (begins && t == 0) {
                         // this CTA holds the first piece: it names the item and where its pieces are
-                        const int64_t end = w1 - part_left + it.blocks;
+                        const int64_t end = w1 - part.left + it.blocks;
                         int64_t last = (end - 1) * ctas / total;
                         while (total * (last + 1) / ctas < end) ++last;
                         while (total * last / ctas > end - 1) --last;
@@ -572,24 +670,28 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 if (any) tc_fence_before();
                 q_scale = next_scale;
+                part_done();
             }
         } else if (warp < 12) {
             // ------------------------------------------------------------------ 8-bit tiles -> fp16 tiles
             const int ct = t - 256;
             uint32_t n = 0;
             bool ok = true, more = true;
-            while (more && ok) {
-                for (int j = walk.step; j < walk.stop && ok; ++j) {
-                    if (!walk.live(j)) continue;
-                    const int valid = walk.it.length - (walk.it.key0 + j * kBlock);       // rows with a token
+            while (more && (ok = ok && part_wait())) {
+                const PromptPart& part = parts[n_part % kPartSlots];
+                more = !part.last;
+                const int live1 = part.live1, tokens = part.it.length - part.it.key0;
+                for (int j = part.live0; j < live1 && ok; ++j) {
+                    const int valid = tokens - j * kBlock;                                // rows with a token
+#pragma unroll 1
                     for (int side = 0; side < 2; ++side, ++n) {
                         const int rs = n % S::kRawRing, slot = n % S::kRing;
-                        ok = warp_wait_bounded(smem_addr(&bars.raw_full[rs]), (n / S::kRawRing) & 1, abort, wait_code(4, rs)) &&
-                             warp_wait_bounded(smem_addr(&bars.empty[slot]), ((n / S::kRing) & 1) ^ 1, abort, wait_code(5, slot));
+                        ok = prompt_wait(smem_addr(&bars.raw_full[rs]), (n / S::kRawRing) & 1, abort, wait_code(4, rs)) &&
+                             prompt_wait(smem_addr(&bars.empty[slot]), ((n / S::kRing) & 1) ^ 1, abort, wait_code(5, slot));
                         if (!ok) break;
                         const uint32_t from = raw + rs * S::kRaw, to = ring + slot * S::kTile;
                         constexpr int CHUNKS = DIM / 16;                                  // 16-byte chunks of a key
-#pragma unroll
+#pragma unroll 2
                         for (int i = 0; i < kBlock * CHUNKS / 128; ++i) {
                             const int g = ct + i * 128, row = g / CHUNKS, c = g % CHUNKS;
                             const uint32_t at = DIM == 64 ? from + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
@@ -624,125 +726,142 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         }
                     }
                 }
-                more = ok && walk.next(p);
+                part_done();
             }
         } else if (warp == 12) {
             // ------------------------------------------------------------------ products
-            if (lane == 0) {
-                const uint32_t idesc_s = f16_idesc(128, kBlock, false), idesc_o = f16_idesc(128, DIM, true);
-                uint32_t n = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-                bool ok = true, more = true;
-                auto wait = [&](uint64_t& bar, uint32_t parity, int role, int index) {
-                    if (ok) ok = wait_bounded(smem_addr(&bar), parity & 1, abort, wait_code(role, index));
-                    tc_fence_after();
-                };
-                auto scores = [&](int tile, uint32_t slot) {
-#pragma unroll
-                    for (int k = 0; k < DIM / 16; ++k) {
-                        const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                        umma_f16(tmem + tile * 128, make_smem_desc(q_smem + tile * (S::kQ / 2) + off, 128),
-                                 make_smem_desc(ring + slot * S::kTile + off, 128), idesc_s, k > 0);
-                    }
-                    umma_commit(smem_addr(&bars.s_full[tile]));
-                };
-                while (more && ok) {
-                    int j = walk.step;
-                    while (j < walk.stop && !walk.live(j)) ++j;
-                    if (j < walk.stop) {
-                        for (int tile = 0; tile < 2 && ok; ++tile)
-                            if (walk.end_of(tile) > walk.first_of(tile)) wait(bars.q_full[tile], q_uses[tile]++, 6, tile);
-                        wait(bars.full[n % S::kRing], n / S::kRing, 7, n % S::kRing);
-                        if (!ok) break;
-                        for (int tile = 0; tile < 2; ++tile)
-                            if (walk.active(tile, j)) scores(tile, n % S::kRing);
-                        umma_commit(smem_addr(&bars.empty[n % S::kRing]));
-                        for (; j < walk.stop && walk.live(j) && ok; ++j, n += 2) {
-                            const uint32_t v = n + 1, k_next = n + 2;
-                            const bool again = j + 1 < walk.stop && walk.live(j + 1);
-                            wait(bars.full[v % S::kRing], v / S::kRing, 8, v % S::kRing);
-                            bool have = false;
-                            for (int tile = 0; tile < 2 && ok; ++tile) {
-                                if (walk.active(tile, j)) {
-                                    wait(bars.p_ready[tile], p_uses[tile]++, 9, tile);
-                                    if (!ok) break;
-                                    const bool first = j == walk.first_of(tile);
-#pragma unroll
-                                    for (int k = 0; k < kBlock / 16; ++k)
-                                        umma_f16_ts(tmem + S::kO + tile * DIM, tmem + tile * 128 + k * 8,
-                                                    mn_desc(ring + (v % S::kRing) * S::kTile + k * 2048, kBlock * 128, 1024),
-                                                    idesc_o, !(first && k == 0));
-                                    if (j + 1 == walk.end_of(tile)) umma_commit(smem_addr(&bars.o_full[tile]));
-                                }
-                                if (again && walk.active(tile, j + 1)) {
-                                    if (!have) wait(bars.full[k_next % S::kRing], k_next / S::kRing, 7, k_next % S::kRing);
-                                    have = true;
-                                    if (!ok) break;
-                                    scores(tile, k_next % S::kRing);
-                                }
-                            }
+            // The whole warp walks along and one elected lane issues: descriptors are then uniform values,
+            // which the instruction takes from uniform registers (from one lane's registers each product
+            // cost over 250 cycles to issue).
+            const uint32_t idesc_s = f16_idesc(128, kBlock, false), idesc_o = f16_idesc(128, DIM, true);
+            uint32_t n = 0, q_uses[2] = {0, 0}, p_uses = 0;              // p_uses: a phase bit for each tile
+            bool ok = true, more = true;
+            const auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+            const uint32_t tm = uniform(tmem);
+            auto wait = [&](uint64_t& bar, uint32_t parity, int role, int index) {
+                if (ok) ok = prompt_wait(smem_addr(&bar), parity & 1, abort, wait_code(role, index));
+                tc_fence_after();
+            };
+            while (more && (ok = ok && part_wait())) {
+                const PromptPart& part = parts[n_part % kPartSlots];
+                more = !part.last;
+                const int live0 = uniform(part.live0), live1 = uniform(part.live1);
+                const int from0 = uniform(part.mine0[0]), to0 = uniform(part.mine1[0]);
+                const int from1 = uniform(part.mine0[1]), to1 = uniform(part.mine1[1]);
+                if (to0 > from0) wait(bars.q_full[0], q_uses[0]++, 6, 0);
+                if (to1 > from1) wait(bars.q_full[1], q_uses[1]++, 6, 1);
+                // Block j's second product, then block j + 1's first into the same columns, tile after tile.
+                // n counts tiles: keys of block j at n, its values at n + 1, the next keys at n + 2.
+#pragma unroll 1
+                for (int j = live0 - 1; j < live1 && live0 < live1; ++j) {
+                    const uint32_t v = (n + 1) % S::kRing;
+                    const bool now = j >= live0, again = j + 1 < live1;
+                    const uint32_t k_index = now ? n + 2 : n, k_next = k_index % S::kRing;
+                    if (now) wait(bars.full[v], (n + 1) / S::kRing, 8, v);
+                    bool have = false;
+#pragma unroll 1
+                    for (int tile = 0; tile < 2 && ok; ++tile) {
+                        const int from = tile ? from1 : from0, to = tile ? to1 : to0;
+                        if (j >= from && j < to) {
+                            wait(bars.p_ready[tile], p_uses >> (tile * 16), 9, tile);
+                            p_uses ^= 1u << (tile * 16);
                             if (!ok) break;
-                            umma_commit(smem_addr(&bars.empty[v % S::kRing]));
-                            if (again) umma_commit(smem_addr(&bars.empty[k_next % S::kRing]));
+                            const uint32_t d = tm + S::kO + tile * DIM, a = tm + tile * 128, first = j == from ? 0 : 1;
+                            const uint64_t b = mn_desc(ring + v * S::kTile, kBlock * 128, 1024);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < kBlock / 16; ++k)
+                                    umma_f16_ts(d, a + k * 8, b + (k * 2048 >> 4), idesc_o, k > 0 ? 1 : first);
+                                if (j + 1 == to) umma_commit(smem_addr(&bars.o_full[tile]));
+                            }
+                            __syncwarp();
+                        }
+                        if (again && j + 1 >= from && j + 1 < to) {
+                            if (!have) wait(bars.full[k_next], k_index / S::kRing, 7, k_next);
+                            have = true;
+                            if (!ok) break;
+                            const uint32_t d = tm + tile * 128;
+                            const uint64_t a = make_smem_desc(q_smem + tile * (S::kQ / 2), 128);
+                            const uint64_t b = make_smem_desc(ring + k_next * S::kTile, 128);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < DIM / 16; ++k) {
+                                    const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                                    umma_f16(d, a + off, b + off, idesc_s, k > 0);
+                                }
+                                umma_commit(smem_addr(&bars.s_full[tile]));
+                            }
+                            __syncwarp();
                         }
                     }
-                    more = ok && walk.next(p);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        if (now) umma_commit(smem_addr(&bars.empty[v]));
+                        if (again) umma_commit(smem_addr(&bars.empty[k_next]));
+                    }
+                    __syncwarp();
+                    if (now) n += 2;
                 }
-                // nothing may still be on its way to this CTA's barriers when it leaves
-                for (uint32_t i = n > S::kRing ? n - S::kRing : 0; i < n && ok; ++i)
-                    wait(bars.empty[i % S::kRing], i / S::kRing, 10, i % S::kRing);
+                if (ok) part_done();
             }
-            __syncwarp();
+            // nothing may still be on its way to this CTA's barriers when it leaves
+            for (uint32_t i = n > S::kRing ? n - S::kRing : 0; i < n && ok; ++i)
+                wait(bars.empty[i % S::kRing], i / S::kRing, 10, i % S::kRing);
         } else if (warp == 13) {
             // ------------------------------------------------------------------ copies
             uint32_t n = 0;
             bool ok = true, more = true;
             const int boxes = kBlock / p.box_rows;
-            while (more && ok) {
-                const PromptItem& it = walk.it;
-                for (int j = walk.step; j < walk.stop && ok; ++j) {
-                    if (!walk.live(j)) continue;
-                    const int key = it.key0 + j * kBlock + lane * p.box_rows;
+            while (more && (ok = ok && part_wait())) {
+                const PromptPart& part = parts[n_part % kPartSlots];
+                more = !part.last;
+                const int live1 = part.live1, b = part.it.b, kv_head = part.it.kv_head, key0 = part.it.key0, length = part.it.length;
+                for (int j = part.live0; j < live1 && ok; ++j) {
+                    const int key = key0 + j * kBlock + lane * p.box_rows;
                     int z = (int)p.c.pages;                            // behind the last page: zeros
-                    if (lane < boxes && key < it.length) {
-                        const int page = kv_page(p.c, it.b, key >> p.c.page_shift);
+                    if (lane < boxes && key < length) {
+                        const int page = kv_page(p.c, b, key >> p.c.page_shift);
                         if (page >= 0) z = page;
                     }
+#pragma unroll 1
                     for (int side = 0; side < 2; ++side, ++n) {
                         const int rs = n % S::kRawRing;
-                        ok = warp_wait_bounded(smem_addr(&bars.raw_empty[rs]), ((n / S::kRawRing) & 1) ^ 1, abort, wait_code(11, rs));
+                        ok = prompt_wait(smem_addr(&bars.raw_empty[rs]), ((n / S::kRawRing) & 1) ^ 1, abort, wait_code(11, rs));
                         if (!ok) break;
                         const uint32_t bar = smem_addr(&bars.raw_full[rs]);
                         if (lane == 0) mbar_arrive_expect_tx(bar, S::kRaw);
                         __syncwarp();
                         if (lane < boxes)
                             tma_load_3d(raw + rs * S::kRaw + lane * p.box_rows * DIM, side ? &map_v : &map_k, bar, 0,
-                                        it.kv_head * p.c.page_tokens + (key & (p.c.page_tokens - 1)), z);
+                                        kv_head * p.c.page_tokens + (key & (p.c.page_tokens - 1)), z);
                     }
                 }
-                more = ok && walk.next(p);
+                part_done();
             }
         } else if (warp == 14) {
             // ------------------------------------------------------------------ scales of the pages
             uint32_t n = 0;
             bool ok = true, more = true;
-            while (more && ok) {
-                const PromptItem& it = walk.it;
+            while (more && (ok = ok && part_wait())) {
+                const PromptPart& part = parts[n_part % kPartSlots];
+                more = !part.last;
+                const int live1 = part.live1, b = part.it.b, kv_head = part.it.kv_head, key0 = part.it.key0;
+                const int length = part.it.length, low = part.it.low;
                 float unit = 0x1p-123f;
-                for (int j = walk.step; j < walk.stop && ok; ++j) {
-                    if (!walk.live(j)) continue;
-                    const int key = it.key0 + j * kBlock + (lane & 7) * 16;
+                for (int j = part.live0; j < live1 && ok; ++j) {
+                    const int key = key0 + j * kBlock + (lane & 7) * 16;
                     float ks = 0.0f, vs = 0.0f;
-                    if (key < it.length) {
-                        const int page = kv_page(p.c, it.b, key >> p.c.page_shift);
+                    if (key < length) {
+                        const int page = kv_page(p.c, b, key >> p.c.page_shift);
                         if (page >= 0) {
-                            const int64_t block = (int64_t)page * p.c.kv_heads + it.kv_head;
+                            const int64_t block = (int64_t)page * p.c.kv_heads + kv_head;
                             ks = p.c.scale[0][block];
                             vs = p.c.scale[1][block];
                         }
                     }
                     if (!(fabsf(vs) <= 3.0e38f)) vs = __uint_as_float(0x7fc00000u);
                     // the largest of the finite ones that some row sees
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, vs == vs && key + 16 > it.low ? __float_as_uint(fabsf(vs)) : 0u);
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, vs == vs && key + 16 > low ? __float_as_uint(fabsf(vs)) : 0u);
                     float ratio = 1.0f;
                     if (__uint_as_float(top) > 16.0f * unit) {
                         const float grown = __uint_as_float(top & 0x7f800000u);
@@ -750,7 +869,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         unit = grown;
                     }
                     const int slot = n % kScaleSlots;
-                    ok = warp_wait_bounded(smem_addr(&bars.scale_empty[slot]), ((n / kScaleSlots) & 1) ^ 1, abort, wait_code(12, slot));
+                    ok = prompt_wait(smem_addr(&bars.scale_empty[slot]), ((n / kScaleSlots) & 1) ^ 1, abort, wait_code(12, slot));
                     if (!ok) break;
                     ++n;
                     if (lane < 8) { scales[slot].key[lane] = ks; scales[slot].weight[lane] = vs / unit; }
@@ -758,7 +877,23 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_addr(&bars.scale_full[slot]));
                 }
-                more = ok && walk.next(p);
+                part_done();
+            }
+        } else if (warp == 15) {
+            // ------------------------------------------------------------------ parts
+            PromptPart part = parts[0];
+            bool ok = true;
+            if (lane == 0) mbar_arrive(smem_addr(&bars.part_full[0]));      // keeps slot 0's phases in step
+            for (uint32_t n = 1; ok && !part.last; ++n) {
+                prompt_next(p, part);
+                const int slot = n % kPartSlots;
+                ok = prompt_wait(smem_addr(&bars.part_empty[slot]), ((n / kPartSlots) & 1) ^ 1, abort, wait_code(14, slot));
+                if (!ok) break;
+                if (lane == 0) {
+                    parts[slot] = part;
+                    mbar_arrive(smem_addr(&bars.part_full[slot]));
+                }
+                __syncwarp();
             }
         }
     }
