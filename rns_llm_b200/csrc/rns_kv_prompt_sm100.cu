@@ -183,26 +183,29 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8])
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+// Two fp32 operations in one instruction; a pair lives in 64 bits.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float x, float y) { return ((Pair)__float_as_uint(y) << 32) | (Pair)__float_as_uint(x); }
+__device__ __forceinline__ float pair_x(Pair p) { return __uint_as_float((uint32_t)p); }
+__device__ __forceinline__ float pair_y(Pair p) { return __uint_as_float((uint32_t)(p >> 32)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
-        "mov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
-        "mov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ float prompt_exp2(float x) {
@@ -271,34 +274,72 @@ struct PromptScales {
     float pad[2];
 };
 
-// 32 of a row's scores -> weights 2^(s f - m), added up in `sum`, and times the values' scale as fp16 to
-// tensor memory.  WHOLE: the row sees every column; otherwise the bits of `seen` say which.
+// Bits [lo, hi) of the 32 columns from `at` on: those a row sees.
+__device__ __forceinline__ uint32_t prompt_seen(int at, int lo, int hi) {
+    const int a = min(max(lo - at, 0), 32), b = min(max(hi - at, 0), 32);
+    return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
+}
+// The largest score of this thread's row of a block, in chunks of 32 columns (a loop, not 128 columns
+// unrolled: see prompt_wait).  WHOLE: the row sees every column, otherwise columns [lo, hi).
 template <bool WHOLE>
-__device__ __forceinline__ void prompt_weights(const float (&s)[32], uint32_t seen, const float* key, const float* weights,
-                                               float q_scale, float m, uint32_t tmem, float2& sum) {
-    const float2 minus_m = make_float2(-m, -m);
-    uint32_t w[16];
+__device__ __forceinline__ float prompt_top(uint32_t s_tmem, const PromptScales& sc, float q_scale, int lo, int hi) {
+    float top = kNoScore;
+#pragma unroll 1
+    for (int ch = 0; ch < 4; ++ch) {
+        float s[32];
+        tmem_ld32(s_tmem + ch * 32, s);
+        tmem_ld_wait();
+        if (!WHOLE) {
+            const uint32_t seen = prompt_seen(ch * 32, lo, hi);
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        const float f = key[g] * q_scale, weight = weights[g];
-        float2 e[8];
+            for (int i = 0; i < 32; ++i)
+                if (!((seen >> i) & 1)) s[i] = -INFINITY;
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = fma2(make_float2(s[g * 16 + 2 * i], s[g * 16 + 2 * i + 1]), make_float2(f, f), minus_m);
+        for (int g = 0; g < 2; ++g) {
+            float best = fmaxf(s[g * 16], s[g * 16 + 15]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = make_float2(prompt_exp2(e[i].x), prompt_exp2(e[i].y));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float2 pw = mul2(e[i], make_float2(weight, weight));
-            if (!WHOLE) {                                           // not NaN from a scale that this row does not see
-                if (!((seen >> (g * 16 + 2 * i)) & 1)) e[i].x = pw.x = 0.0f;
-                if (!((seen >> (g * 16 + 2 * i + 1)) & 1)) e[i].y = pw.y = 0.0f;
-            }
-            sum = add2(sum, e[i]);
-            const __half2 h = __floats2half2_rn(pw.x, pw.y);
-            w[g * 8 + i] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int i = 1; i < 15; i += 2) best = max3(best, s[g * 16 + i], s[g * 16 + i + 1]);
+            top = fmaxf(top, best * (sc.key[ch * 2 + g] * q_scale));
         }
     }
-    tmem_st16(tmem, w);
+    return top;
+}
+// Scores -> weights 2^(s f - m), whose sum is returned, and times the values' scale as fp16 into the place of
+// the scores.
+template <bool WHOLE>
+__device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const PromptScales& sc, float q_scale, float m, int lo, int hi) {
+    const Pair minus_m = pair(-m, -m);
+    Pair sum = pair(0.0f, 0.0f);
+#pragma unroll 1
+    for (int ch = 0; ch < 4; ++ch) {
+        float s[32];
+        tmem_ld32(s_tmem + ch * 32, s);
+        tmem_ld_wait();
+        const uint32_t seen = WHOLE ? 0 : prompt_seen(ch * 32, lo, hi);
+        uint32_t w[16];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const float f = sc.key[ch * 2 + g] * q_scale, weight = sc.weight[ch * 2 + g];
+            const Pair f2 = pair(f, f), weight2 = pair(weight, weight);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const Pair x = fma2(pair(s[g * 16 + 2 * i], s[g * 16 + 2 * i + 1]), f2, minus_m);
+                Pair e = pair(prompt_exp2(pair_x(x)), prompt_exp2(pair_y(x)));
+                Pair pw = mul2(e, weight2);
+                if (!WHOLE) {                                       // not NaN from a scale that this row does not see
+                    const bool a = (seen >> (g * 16 + 2 * i)) & 1, b = (seen >> (g * 16 + 2 * i + 1)) & 1;
+                    e = pair(a ? pair_x(e) : 0.0f, b ? pair_y(e) : 0.0f);
+                    pw = pair(a ? pair_x(pw) : 0.0f, b ? pair_y(pw) : 0.0f);
+                }
+                sum = add2(sum, e);
+                const __half2 h = __floats2half2_rn(pair_x(pw), pair_y(pw));
+                w[g * 8 + i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        tmem_st16(s_tmem + ch * 16, w);
+    }
+    return pair_x(sum) + pair_y(sum);
 }
 
 template <int DIM, int FORMAT>
@@ -515,32 +556,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     const int key = key0 + j * kBlock;
                     const bool whole = key + kBlock <= all_hi && key >= all_lo;
                     const int col_lo = lo - key, col_hi = hi - key;
-                    // bits [col_lo, col_hi) of a chunk's 32 columns: those this row sees
-                    const auto seen = [&](int ch) {
-                        const int a = min(max(col_lo - ch * 32, 0), 32), b = min(max(col_hi - ch * 32, 0), 32);
-                        return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
-                    };
-                    // this row's largest score
-                    float top = kNoScore;
-#pragma unroll 1
-                    for (int ch = 0; ch < 4; ++ch) {
-                        float s[32];
-                        tmem_ld32(s_tmem + ch * 32, s);
-                        tmem_ld_wait();
-                        if (!whole) {
-                            const uint32_t bits = seen(ch);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (!((bits >> i) & 1)) s[i] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            float best = s[g * 16];
-#pragma unroll
-                            for (int i = 1; i < 16; ++i) best = fmaxf(best, s[g * 16 + i]);
-                            top = fmaxf(top, best * (sc.key[ch * 2 + g] * q_scale));
-                        }
-                    }
+                    float top = whole ? prompt_top<true>(s_tmem, sc, q_scale, 0, 0) : prompt_top<false>(s_tmem, sc, q_scale, col_lo, col_hi);
                     const bool first = j == mine0;
                     if (!(top > m + kScoreLag)) top = m;
                     const float keep = prompt_exp2(m - top), ratio = sc.ratio;
@@ -561,16 +577,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         }
                     }
                     // weights, in place of the scores
-                    float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll 1
-                    for (int ch = 0; ch < 4; ++ch) {
-                        float s[32];
-                        tmem_ld32(s_tmem + ch * 32, s);
-                        tmem_ld_wait();
-                        if (whole) prompt_weights<true>(s, 0, &sc.key[ch * 2], &sc.weight[ch * 2], q_scale, m, s_tmem + ch * 16, sum);
-                        else prompt_weights<false>(s, seen(ch), &sc.key[ch * 2], &sc.weight[ch * 2], q_scale, m, s_tmem + ch * 16, sum);
-                    }
-                    l += sum.x + sum.y;
+                    l += whole ? prompt_weights<true>(s_tmem, sc, q_scale, m, 0, 0) : prompt_weights<false>(s_tmem, sc, q_scale, m, col_lo, col_hi);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -674,7 +681,11 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             }
         } else if (warp < 12) {
             // ------------------------------------------------------------------ 8-bit tiles -> fp16 tiles
-            const int ct = t - 256;
+            const int lane_key = ((lane >> 3) & 3) ^ (((lane >> 2) & 1) * 5), lane_chunk = lane & 3;
+            // byte of this lane's chunk in 8 keys as TMA swizzled them, and of its two chunks in a part of the fp16 tile
+            const uint32_t raw_at = DIM == 64 ? lane_key * 64 + ((lane_chunk ^ ((lane_key >> 1) & 3)) << 4)
+                                              : lane_key * 128 + ((lane_chunk ^ (lane_key & 3)) << 4);
+            const uint32_t raw_flip = (lane_key & 4) << 4, out0 = ((2 * lane_chunk) ^ lane_key) << 4;
             uint32_t n = 0;
             bool ok = true, more = true;
             while (more && (ok = ok && part_wait())) {
@@ -690,33 +701,26 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                              prompt_wait(smem_addr(&bars.empty[slot]), ((n / S::kRing) & 1) ^ 1, abort, wait_code(5, slot));
                         if (!ok) break;
                         const uint32_t from = raw + rs * S::kRaw, to = ring + slot * S::kTile;
-                        constexpr int CHUNKS = DIM / 16;                                  // 16-byte chunks of a key
+                        // Units of 8 keys x 64 dimensions, one 16-byte chunk a lane.  Eight neighbouring lanes hold
+                        // four chunks of keys k and k ^ 5, whose swizzles differ in bits 0 and 2: neither the
+                        // 16-byte loads nor the stores meet a bank twice, and every swizzle is a constant of the lane.
 #pragma unroll 2
-                        for (int i = 0; i < kBlock * CHUNKS / 128; ++i) {
-                            const int g = ct + i * 128, row = g / CHUNKS, c = g % CHUNKS;
-                            const uint32_t at = DIM == 64 ? from + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
-                                                          : from + row * 128 + ((c ^ (row & 7)) << 4);
+                        for (int u = warp - 8; u < kBlock / 8 * S::kParts; u += 4) {
+                            const int part64 = u % S::kParts, keys = u / S::kParts * 8;
+                            const uint32_t at = from + keys * DIM + raw_at + (DIM == 128 ? (part64 << 6 ^ raw_flip) : 0);
                             uint32_t w[4];
                             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
                             // bytes behind the sequence may be NaN patterns, which no weight of zero removes
-                            if (FORMAT == RNS_KV_E4M3 && row >= valid) w[0] = w[1] = w[2] = w[3] = 0;
+                            if (FORMAT == RNS_KV_E4M3 && keys + lane_key >= valid) w[0] = w[1] = w[2] = w[3] = 0;
                             uint32_t h[8];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 if (FORMAT == RNS_KV_INT8) { h[2 * k] = half_pair_s8(w[k]); h[2 * k + 1] = half_pair_s8(w[k] >> 8); }
                                 else { h[2 * k] = half_pair_e4m3(w[k]); h[2 * k + 1] = half_pair_e4m3(w[k] >> 16); }
                             }
-                            const uint32_t out = to + (c >> 2) * (kBlock * 128) + row * 128;
-                            const int c0 = 2 * (c & 3);
-                            // eight lanes hold one key of two parts: the upper part stores its second half first (banks)
-                            const bool swap = DIM == 128 && c >= 4;
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const int half = swap ? 1 - k : k;
-                                const uint32_t dst = out + (((c0 + half) ^ (row & 7)) << 4);
-                                const uint32_t a0 = half ? h[4] : h[0], a1 = half ? h[5] : h[1], a2 = half ? h[6] : h[2], a3 = half ? h[7] : h[3];
-                                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(a0), "r"(a1), "r"(a2), "r"(a3) : "memory");
-                            }
+                            const uint32_t out = to + part64 * (kBlock * 128) + keys * 128 + lane_key * 128;
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(out + out0), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(out + (out0 ^ 16)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
