@@ -30,11 +30,15 @@
 namespace rns {
 
 constexpr int kPromptThreads = 512;
-constexpr int kBlock = 128;               // keys of a block
+constexpr int kBlock = 128, kHalf = 64;   // keys of a block, and of the halves it is exponentiated in
 constexpr int kTileRows = 128;
 constexpr float kNoScore = -1.7e38f;      // below every score: "nothing seen yet"
 constexpr float kScoreLag = 8.0f;
 constexpr int kScaleSlots = 4, kPartSlots = 4;
+// Registers: a softmax thread holds half of its row's scores of a block.  Two warpgroups of kSoftmaxRegs and
+// two of kOtherRegs must not exceed what the block was launched with, 512 threads x kLaunchRegs.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
 
 struct PromptParams {
     KvView c;
@@ -239,33 +243,31 @@ __device__ __forceinline__ uint32_t half_pair_e4m3(uint32_t x) {
     return r;
 }
 
-// Waits of whole warps.  Sixteen warps run eight different programs here, and the instruction cache is
-// what they compete for first (inlined waits and fully unrolled rows of 128 columns made "no
-// instruction" the largest stall by far): the waiting itself is one function for all of them.
-__device__ __noinline__ bool prompt_wait_long(uint32_t bar, uint32_t parity, volatile int* abort, int where) {
-    const long long t0 = clock64();
-    for (uint32_t spin = 1;; ++spin) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((spin & 255u) == 0) {
-            if (*abort) return false;
-            if (clock64() - t0 > kWaitLimitCycles) {
-                if (*abort == 0) *abort = where;
-                return false;
-            }
-        }
-    }
-}
+// Waits of whole warps, bounded by about a second of SM clock.  Sixteen warps run eight different programs
+// here, and the instruction cache is what they compete for first: with waits of 64 inlined polls and rows of
+// 128 columns unrolled in two forms, "no instruction" was the largest stall by far.
 __device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity, volatile int* abort, int where) {
     bool ok = mbar_try_wait(bar, parity);
     if (!__all_sync(0xffffffffu, ok)) {
-        if (!ok) ok = prompt_wait_long(bar, parity, abort, where);
+        const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+        for (uint32_t spin = 1; !ok; ++spin) {
+            ok = mbar_try_wait(bar, parity);
+            if (!ok && (spin & 255u) == 0) {
+                if (*abort) break;
+                if ((uint32_t)clock() - t0 > 2000000000u) {
+                    if (*abort == 0) *abort = where;
+                    break;
+                }
+            }
+        }
         ok = __all_sync(0xffffffffu, ok);
     }
     return ok;
 }
 
 struct PromptBars {
-    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2], o_full[2], q_full[2];
+    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2][2], p_ready[2][2], o_done[2][2], q_full[2];
     uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots], part_full[kPartSlots], part_empty[kPartSlots];
 };
 struct PromptScales {
@@ -279,65 +281,45 @@ __device__ __forceinline__ uint32_t prompt_seen(int at, int lo, int hi) {
     const int a = min(max(lo - at, 0), 32), b = min(max(hi - at, 0), 32);
     return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
 }
-// The largest score of this thread's row of a block, in chunks of 32 columns (a loop, not 128 columns
-// unrolled: see prompt_wait).  WHOLE: the row sees every column, otherwise columns [lo, hi).
-template <bool WHOLE>
-__device__ __forceinline__ float prompt_top(uint32_t s_tmem, const PromptScales& sc, float q_scale, int lo, int hi) {
+// The largest score of a row's half block; key: scales of its four groups of 16 keys.
+__device__ __forceinline__ float prompt_top(const float (&s)[kHalf], const float* key, float q_scale) {
     float top = kNoScore;
-#pragma unroll 1
-    for (int ch = 0; ch < 4; ++ch) {
-        float s[32];
-        tmem_ld32(s_tmem + ch * 32, s);
-        tmem_ld_wait();
-        if (!WHOLE) {
-            const uint32_t seen = prompt_seen(ch * 32, lo, hi);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (!((seen >> i) & 1)) s[i] = -INFINITY;
-        }
+    for (int g = 0; g < kHalf / 16; ++g) {
+        float best = fmaxf(s[g * 16], s[g * 16 + 15]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            float best = fmaxf(s[g * 16], s[g * 16 + 15]);
-#pragma unroll
-            for (int i = 1; i < 15; i += 2) best = max3(best, s[g * 16 + i], s[g * 16 + i + 1]);
-            top = fmaxf(top, best * (sc.key[ch * 2 + g] * q_scale));
-        }
+        for (int i = 1; i < 15; i += 2) best = max3(best, s[g * 16 + i], s[g * 16 + i + 1]);
+        top = fmaxf(top, best * (key[g] * q_scale));
     }
     return top;
 }
 // Scores -> weights 2^(s f - m), whose sum is returned, and times the values' scale as fp16 into the place of
-// the scores.
+// the scores.  WHOLE: the row sees every column; otherwise the bits of `seen` say which.
 template <bool WHOLE>
-__device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const PromptScales& sc, float q_scale, float m, int lo, int hi) {
+__device__ __forceinline__ float prompt_weights(const float (&s)[kHalf], const uint32_t (&seen)[2], uint32_t s_tmem,
+                                                const float* key, const float* weights, float q_scale, float m) {
     const Pair minus_m = pair(-m, -m);
     Pair sum = pair(0.0f, 0.0f);
-#pragma unroll 1
-    for (int ch = 0; ch < 4; ++ch) {
-        float s[32];
-        tmem_ld32(s_tmem + ch * 32, s);
-        tmem_ld_wait();
-        const uint32_t seen = WHOLE ? 0 : prompt_seen(ch * 32, lo, hi);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
         uint32_t w[16];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const float f = sc.key[ch * 2 + g] * q_scale, weight = sc.weight[ch * 2 + g];
-            const Pair f2 = pair(f, f), weight2 = pair(weight, weight);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const Pair x = fma2(pair(s[g * 16 + 2 * i], s[g * 16 + 2 * i + 1]), f2, minus_m);
-                Pair e = pair(prompt_exp2(pair_x(x)), prompt_exp2(pair_y(x)));
-                Pair pw = mul2(e, weight2);
-                if (!WHOLE) {                                       // not NaN from a scale that this row does not see
-                    const bool a = (seen >> (g * 16 + 2 * i)) & 1, b = (seen >> (g * 16 + 2 * i + 1)) & 1;
-                    e = pair(a ? pair_x(e) : 0.0f, b ? pair_y(e) : 0.0f);
-                    pw = pair(a ? pair_x(pw) : 0.0f, b ? pair_y(pw) : 0.0f);
-                }
-                sum = add2(sum, e);
-                const __half2 h = __floats2half2_rn(pair_x(pw), pair_y(pw));
-                w[g * 8 + i] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int i = 0; i < 16; ++i) {
+            const int g = c * 2 + (i >> 3), col = c * 32 + 2 * i;
+            const float f = key[g] * q_scale, weight = weights[g];
+            const Pair x = fma2(pair(s[col], s[col + 1]), pair(f, f), minus_m);
+            Pair e = pair(prompt_exp2(pair_x(x)), prompt_exp2(pair_y(x)));
+            Pair pw = mul2(e, pair(weight, weight));
+            if (!WHOLE) {                                           // not NaN from a scale that this row does not see
+                const bool a = (seen[c] >> (2 * i)) & 1, b = (seen[c] >> (2 * i + 1)) & 1;
+                e = pair(a ? pair_x(e) : 0.0f, b ? pair_y(e) : 0.0f);
+                pw = pair(a ? pair_x(pw) : 0.0f, b ? pair_y(pw) : 0.0f);
             }
+            sum = add2(sum, e);
+            const __half2 h = __floats2half2_rn(pair_x(pw), pair_y(pw));
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        tmem_st16(s_tmem + ch * 16, w);
+        tmem_st16(s_tmem + c * 16, w);
     }
     return pair_x(sum) + pair_y(sum);
 }
@@ -366,9 +348,11 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             mbar_init(smem_addr(&bars.empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&bars.s_full[i]), 1);
-            mbar_init(smem_addr(&bars.p_ready[i]), 4);
-            mbar_init(smem_addr(&bars.o_full[i]), 1);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(smem_addr(&bars.s_full[i][h]), 1);
+                mbar_init(smem_addr(&bars.p_ready[i][h]), 4);
+                mbar_init(smem_addr(&bars.o_done[i][h]), 1);
+            }
             mbar_init(smem_addr(&bars.q_full[i]), 4);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
@@ -451,11 +435,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
         if (warp < 8) {
             // ------------------------------------------------------------------ softmax
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t s_tmem = tmem + tile * 128 + lanes, o_tmem = tmem + S::kO + tile * DIM + lanes;
             const int row_token = row / p.head_tile, row_head = row - row_token * p.head_tile;
-            uint32_t s_uses = 0, o_uses = 0, scale_uses = 0;
+            uint32_t blocks_seen = 0, scale_uses = 0;
 
             // This row's query to shared memory as fp16 times a power of two; returns what the scores are times.
             auto load_q = [&](const PromptItem& it) -> float {
@@ -548,43 +533,63 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         if (lane == 0) mbar_arrive(smem_addr(&bars.scale_empty[slot]));
                         continue;
                     }
-                    ok = prompt_wait(smem_addr(&bars.s_full[tile]), s_uses & 1, abort, wait_code(2, tile));
-                    ++s_uses;
-                    if (!ok) break;
-                    tc_fence_after();
                     const PromptScales& sc = scales[slot];
-                    const int key = key0 + j * kBlock;
-                    const bool whole = key + kBlock <= all_hi && key >= all_lo;
-                    const int col_lo = lo - key, col_hi = hi - key;
-                    float top = whole ? prompt_top<true>(s_tmem, sc, q_scale, 0, 0) : prompt_top<false>(s_tmem, sc, q_scale, col_lo, col_hi);
-                    const bool first = j == mine0;
-                    if (!(top > m + kScoreLag)) top = m;
-                    const float keep = prompt_exp2(m - top), ratio = sc.ratio;
-                    m = top;
+                    const float ratio = sc.ratio;
                     unit = sc.unit;
-                    if (!first && __any_sync(0xffffffffu, keep != 1.0f || ratio != 1.0f)) {
-                        // S(j) has arrived, so the product of the block before has: O is at rest
-                        l *= keep;
 #pragma unroll 1
-                        for (int ch = 0; ch < DIM / 16; ++ch) {
-                            float o[16];
-                            uint32_t v[16];
-                            tmem_ld16(o_tmem + ch * 16, o);
-                            tmem_ld_wait();
+                    for (int half = 0; half < 2; ++half) {
+                        ok = prompt_wait(smem_addr(&bars.s_full[tile][half]), blocks_seen & 1, abort, wait_code(2, tile));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t s_half = s_tmem + half * kHalf;
+                        const float *key_scales = sc.key + half * 4, *weights = sc.weight + half * 4;
+                        const int key = key0 + j * kBlock + half * kHalf;
+                        const bool whole = key + kHalf <= all_hi && key >= all_lo;
+                        float s[kHalf];
+                        tmem_ld32(s_half, s);
+                        tmem_ld32(s_half + 32, s + 32);
+                        tmem_ld_wait();
+                        uint32_t seen[2] = {0, 0};
+                        if (!whole) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[i] * (keep * ratio));
-                            tmem_st16(o_tmem + ch * 16, v);
+                            for (int c = 0; c < 2; ++c) {
+                                seen[c] = prompt_seen(c * 32, lo - key, hi - key);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (!((seen[c] >> i) & 1)) s[c * 32 + i] = -INFINITY;
+                            }
                         }
+                        float top = prompt_top(s, key_scales, q_scale);
+                        if (!(top > m + kScoreLag)) top = m;
+                        const float keep = prompt_exp2(m - top), change = half == 0 ? keep * ratio : keep;
+                        m = top;
+                        if (__any_sync(0xffffffffu, keep != 1.0f || change != 1.0f) && (half > 0 || j > mine0)) {
+                            // O must be at rest: the product of the half before may not be finished
+                            ok = prompt_wait(smem_addr(&bars.o_done[tile][half ^ 1]), (blocks_seen - (half ^ 1)) & 1, abort, wait_code(3, tile));
+                            if (!ok) break;
+                            tc_fence_after();
+                            l *= keep;
+#pragma unroll 1
+                            for (int ch = 0; ch < DIM / 16; ++ch) {
+                                float o[16];
+                                uint32_t v[16];
+                                tmem_ld16(o_tmem + ch * 16, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[i] * change);
+                                tmem_st16(o_tmem + ch * 16, v);
+                            }
+                        }
+                        l += whole ? prompt_weights<true>(s, seen, s_half, key_scales, weights, q_scale, m)
+                                   : prompt_weights<false>(s, seen, s_half, key_scales, weights, q_scale, m);
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_addr(&bars.p_ready[tile][half]));
                     }
-                    // weights, in place of the scores
-                    l += whole ? prompt_weights<true>(s_tmem, sc, q_scale, m, 0, 0) : prompt_weights<false>(s_tmem, sc, q_scale, m, col_lo, col_hi);
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_addr(&bars.scale_empty[slot]));
-                        mbar_arrive(smem_addr(&bars.p_ready[tile]));
-                    }
+                    if (!ok) break;
+                    ++blocks_seen;
+                    if (lane == 0) mbar_arrive(smem_addr(&bars.scale_empty[slot]));
                 }
                 if (!ok) break;
                 // the next part's queries before this one's output: their products can start meanwhile
@@ -600,8 +605,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 const bool any = mine1 > mine0;
                 if (any) {
-                    ok = prompt_wait(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
-                    ++o_uses;
+                    ok = prompt_wait(smem_addr(&bars.o_done[tile][0]), (blocks_seen - 1) & 1, abort, wait_code(3, tile)) &&
+                         prompt_wait(smem_addr(&bars.o_done[tile][1]), (blocks_seen - 1) & 1, abort, wait_code(3, tile));
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -679,7 +684,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 q_scale = next_scale;
                 part_done();
             }
-        } else if (warp < 12) {
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        }
+        if (warp >= 8 && warp < 12) {
             // ------------------------------------------------------------------ 8-bit tiles -> fp16 tiles
             const int lane_key = ((lane >> 3) & 3) ^ (((lane >> 2) & 1) * 5), lane_chunk = lane & 3;
             // byte of this lane's chunk in 8 keys as TMA swizzled them, and of its two chunks in a part of the fp16 tile
@@ -737,8 +745,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             // The whole warp walks along and one elected lane issues: descriptors are then uniform values,
             // which the instruction takes from uniform registers (from one lane's registers each product
             // cost over 250 cycles to issue).
-            const uint32_t idesc_s = f16_idesc(128, kBlock, false), idesc_o = f16_idesc(128, DIM, true);
-            uint32_t n = 0, q_uses[2] = {0, 0}, p_uses = 0;              // p_uses: a phase bit for each tile
+            const uint32_t idesc_s = f16_idesc(128, kHalf, false), idesc_o = f16_idesc(128, DIM, true);
+            uint32_t n = 0, q_uses[2] = {0, 0}, p_uses = 0;              // p_uses: a phase bit for each tile's half
             bool ok = true, more = true;
             const auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
             const uint32_t tm = uniform(tmem);
@@ -754,7 +762,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int from1 = uniform(part.mine0[1]), to1 = uniform(part.mine1[1]);
                 if (to0 > from0) wait(bars.q_full[0], q_uses[0]++, 6, 0);
                 if (to1 > from1) wait(bars.q_full[1], q_uses[1]++, 6, 1);
-                // Block j's second product, then block j + 1's first into the same columns, tile after tile.
+                // Half by half: block j's second product, then block j + 1's first into the same columns, tile
+                // after tile, so that the other half's scores are there while one is exponentiated.
                 // n counts tiles: keys of block j at n, its values at n + 1, the next keys at n + 2.
 #pragma unroll 1
                 for (int j = live0 - 1; j < live1 && live0 < live1; ++j) {
@@ -762,38 +771,37 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     const bool now = j >= live0, again = j + 1 < live1;
                     const uint32_t k_index = now ? n + 2 : n, k_next = k_index % S::kRing;
                     if (now) wait(bars.full[v], (n + 1) / S::kRing, 8, v);
-                    bool have = false;
+                    if (again) wait(bars.full[k_next], k_index / S::kRing, 7, k_next);
 #pragma unroll 1
-                    for (int tile = 0; tile < 2 && ok; ++tile) {
+                    for (int step = 0; step < 4 && ok; ++step) {
+                        const int tile = step & 1, half = step >> 1;
                         const int from = tile ? from1 : from0, to = tile ? to1 : to0;
                         if (j >= from && j < to) {
-                            wait(bars.p_ready[tile], p_uses >> (tile * 16), 9, tile);
-                            p_uses ^= 1u << (tile * 16);
+                            wait(bars.p_ready[tile][half], p_uses >> (step * 8), 9, step);
+                            p_uses ^= 1u << (step * 8);
                             if (!ok) break;
-                            const uint32_t d = tm + S::kO + tile * DIM, a = tm + tile * 128, first = j == from ? 0 : 1;
-                            const uint64_t b = mn_desc(ring + v * S::kTile, kBlock * 128, 1024);
+                            const uint32_t d = tm + S::kO + tile * DIM, a = tm + tile * 128 + half * kHalf;
+                            const uint32_t first = j == from && half == 0 ? 0 : 1;
+                            const uint64_t b = mn_desc(ring + v * S::kTile + half * (kHalf * 128), kBlock * 128, 1024);
                             if (elect_one()) {
 #pragma unroll
-                                for (int k = 0; k < kBlock / 16; ++k)
+                                for (int k = 0; k < kHalf / 16; ++k)
                                     umma_f16_ts(d, a + k * 8, b + (k * 2048 >> 4), idesc_o, k > 0 ? 1 : first);
-                                if (j + 1 == to) umma_commit(smem_addr(&bars.o_full[tile]));
+                                umma_commit(smem_addr(&bars.o_done[tile][half]));
                             }
                             __syncwarp();
                         }
                         if (again && j + 1 >= from && j + 1 < to) {
-                            if (!have) wait(bars.full[k_next], k_index / S::kRing, 7, k_next);
-                            have = true;
-                            if (!ok) break;
-                            const uint32_t d = tm + tile * 128;
+                            const uint32_t d = tm + tile * 128 + half * kHalf;
                             const uint64_t a = make_smem_desc(q_smem + tile * (S::kQ / 2), 128);
-                            const uint64_t b = make_smem_desc(ring + k_next * S::kTile, 128);
+                            const uint64_t b = make_smem_desc(ring + k_next * S::kTile + half * (kHalf * 128), 128);
                             if (elect_one()) {
 #pragma unroll
                                 for (int k = 0; k < DIM / 16; ++k) {
                                     const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
                                     umma_f16(d, a + off, b + off, idesc_s, k > 0);
                                 }
-                                umma_commit(smem_addr(&bars.s_full[tile]));
+                                umma_commit(smem_addr(&bars.s_full[tile][half]));
                             }
                             __syncwarp();
                         }
@@ -976,6 +984,9 @@ template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* w
     p.meta = static_cast<int32_t*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)sms * 32);
     const auto kernel = kv_prompt_kernel<DIM, FORMAT>;
+    // the kernel's own split of the registers counts on this launch (looked up once per process)
+    static const int regs = [&] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0; }();
+    if (regs < kLaunchRegs) return fail(RNS_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, not %d", regs, kLaunchRegs);
     RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     kernel<<<sms, kPromptThreads, S::kSmem, st>>>(maps[0], maps[1], p);
     RNS_CUDA_OK(cudaGetLastError());
