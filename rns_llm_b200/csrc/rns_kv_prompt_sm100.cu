@@ -22,23 +22,21 @@
 // * Work is cut as there: one axis of key blocks over all items, equal shares, pieces joined by a
 //   second kernel.
 //
-// Warps 0-3 and 4-7: softmax of a tile (and its queries and outputs); 8-11: conversion; 12: issues the
-// products; 13: copies; 14: scales of the pages; 15: the list of what there is to do.
+// Warps 0-15: softmax (four a tile and half of the block's keys: one thread for a row and half; the same
+// warps fetch the queries and store the outputs, half of the dimensions each); 16-19: conversion; 20: issues
+// the products; 21: copies; 22: scales of the pages; 23: the list of what there is to do.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 
 namespace rns {
 
-constexpr int kPromptThreads = 512;
-constexpr int kBlock = 128, kHalf = 64;   // keys of a block, and of the halves it is exponentiated in
+constexpr int kPromptThreads = 768;
+constexpr int kConvertWarp = 16, kProductWarp = 20, kCopyWarp = 21, kScaleWarp = 22, kPartWarp = 23;
+constexpr int kBlock = 128, kHalf = 64;   // keys of a block, and of the halves that a softmax thread takes
 constexpr int kTileRows = 128;
 constexpr float kNoScore = -1.7e38f;      // below every score: "nothing seen yet"
 constexpr float kScoreLag = 8.0f;
 constexpr int kScaleSlots = 4, kPartSlots = 4;
-// Registers: a softmax thread holds half of its row's scores of a block.  Two warpgroups of kSoftmaxRegs and
-// two of kOtherRegs must not exceed what the block was launched with, 512 threads x kLaunchRegs.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kOtherRegs = 88;
-static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
 
 struct PromptParams {
     KvView c;
@@ -144,7 +142,7 @@ template <int DIM> struct PromptShape {
     static constexpr int kParts = DIM / 64;                        // 64-dimension parts of a tile
     static constexpr int kTile = kBlock * DIM * 2;                 // fp16 tile of keys or values
     static constexpr int kRaw = kBlock * DIM;                      // the same in 8 bits
-    static constexpr int kRing = 4, kRawRing = DIM == 64 ? 4 : 2;
+    static constexpr int kRing = DIM == 64 ? 4 : 3, kRawRing = DIM == 64 ? 4 : 3;
     static constexpr int kQ = 2 * kTileRows * DIM * 2;
     static constexpr int kSmem = 1024 + kQ + kRing * kTile + kRawRing * kRaw;
     static constexpr int kPartial = 2 * kTileRows * (DIM + 2);
@@ -267,7 +265,7 @@ __device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity, volat
 }
 
 struct PromptBars {
-    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2][2], p_ready[2][2], o_done[2][2], q_full[2];
+    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2][2], o_full[2], q_full[2], meet[2][4];
     uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots], part_full[kPartSlots], part_empty[kPartSlots];
 };
 struct PromptScales {
@@ -281,37 +279,51 @@ __device__ __forceinline__ uint32_t prompt_seen(int at, int lo, int hi) {
     const int a = min(max(lo - at, 0), 32), b = min(max(hi - at, 0), 32);
     return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
 }
-// The largest score of a row's half block; key: scales of its four groups of 16 keys.
-__device__ __forceinline__ float prompt_top(const float (&s)[kHalf], const float* key, float q_scale) {
+// The largest score of a row's half block, 16 columns (a page's or part of one) at a time; key: their scales.
+// WHOLE: the row sees every column, otherwise columns [lo, hi).
+template <bool WHOLE>
+__device__ __forceinline__ float prompt_top(uint32_t s_tmem, const float* key, float q_scale, int lo, int hi) {
     float top = kNoScore;
-#pragma unroll
+#pragma unroll 1
     for (int g = 0; g < kHalf / 16; ++g) {
-        float best = fmaxf(s[g * 16], s[g * 16 + 15]);
+        float s[16];
+        tmem_ld16(s_tmem + g * 16, s);
+        tmem_ld_wait();
+        if (!WHOLE) {
+            const uint32_t seen = prompt_seen(g * 16, lo, hi);
 #pragma unroll
-        for (int i = 1; i < 15; i += 2) best = max3(best, s[g * 16 + i], s[g * 16 + i + 1]);
+            for (int i = 0; i < 16; ++i)
+                if (!((seen >> i) & 1)) s[i] = -INFINITY;
+        }
+        float best = fmaxf(s[0], s[15]);
+#pragma unroll
+        for (int i = 1; i < 15; i += 2) best = max3(best, s[i], s[i + 1]);
         top = fmaxf(top, best * (key[g] * q_scale));
     }
     return top;
 }
 // Scores -> weights 2^(s f - m), whose sum is returned, and times the values' scale as fp16 into the place of
-// the scores.  WHOLE: the row sees every column; otherwise the bits of `seen` say which.
+// the scores.
 template <bool WHOLE>
-__device__ __forceinline__ float prompt_weights(const float (&s)[kHalf], const uint32_t (&seen)[2], uint32_t s_tmem,
-                                                const float* key, const float* weights, float q_scale, float m) {
+__device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const float* key, const float* weights, float q_scale,
+                                                float m, int lo, int hi) {
     const Pair minus_m = pair(-m, -m);
     Pair sum = pair(0.0f, 0.0f);
+#pragma unroll 1
+    for (int g = 0; g < kHalf / 16; ++g) {
+        float s[16];
+        tmem_ld16(s_tmem + g * 16, s);
+        const float f = key[g] * q_scale, weight = weights[g];
+        const uint32_t seen = WHOLE ? 0 : prompt_seen(g * 16, lo, hi);
+        uint32_t w[8];
+        tmem_ld_wait();
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int g = c * 2 + (i >> 3), col = c * 32 + 2 * i;
-            const float f = key[g] * q_scale, weight = weights[g];
-            const Pair x = fma2(pair(s[col], s[col + 1]), pair(f, f), minus_m);
+        for (int i = 0; i < 8; ++i) {
+            const Pair x = fma2(pair(s[2 * i], s[2 * i + 1]), pair(f, f), minus_m);
             Pair e = pair(prompt_exp2(pair_x(x)), prompt_exp2(pair_y(x)));
             Pair pw = mul2(e, pair(weight, weight));
             if (!WHOLE) {                                           // not NaN from a scale that this row does not see
-                const bool a = (seen[c] >> (2 * i)) & 1, b = (seen[c] >> (2 * i + 1)) & 1;
+                const bool a = (seen >> (2 * i)) & 1, b = (seen >> (2 * i + 1)) & 1;
                 e = pair(a ? pair_x(e) : 0.0f, b ? pair_y(e) : 0.0f);
                 pw = pair(a ? pair_x(pw) : 0.0f, b ? pair_y(pw) : 0.0f);
             }
@@ -319,7 +331,7 @@ __device__ __forceinline__ float prompt_weights(const float (&s)[kHalf], const u
             const __half2 h = __floats2half2_rn(pair_x(pw), pair_y(pw));
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        tmem_st16(s_tmem + c * 16, w);
+        tmem_st8(s_tmem + g * 8, w);
     }
     return pair_x(sum) + pair_y(sum);
 }
@@ -336,6 +348,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __shared__ __align__(16) PromptScales scales[kScaleSlots];
     __shared__ int64_t scan[kPromptThreads / 32];
     __shared__ PromptPart parts[kPartSlots];
+    __shared__ float met[2][2][2][kTileRows];                      // [turn][tile][half][row]
     __shared__ int abort_word;
     __shared__ uint32_t tmem_holder;
 
@@ -348,25 +361,24 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             mbar_init(smem_addr(&bars.empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            for (int h = 0; h < 2; ++h) {
-                mbar_init(smem_addr(&bars.s_full[i][h]), 1);
-                mbar_init(smem_addr(&bars.p_ready[i][h]), 4);
-                mbar_init(smem_addr(&bars.o_done[i][h]), 1);
-            }
-            mbar_init(smem_addr(&bars.q_full[i]), 4);
+            mbar_init(smem_addr(&bars.s_full[i]), 1);
+            mbar_init(smem_addr(&bars.o_full[i]), 1);
+            for (int h = 0; h < 2; ++h) mbar_init(smem_addr(&bars.p_ready[i][h]), 4);
+            for (int h = 0; h < 4; ++h) mbar_init(smem_addr(&bars.meet[i][h]), 2);
+            mbar_init(smem_addr(&bars.q_full[i]), 8);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
             mbar_init(smem_addr(&bars.scale_full[i]), 1);
-            mbar_init(smem_addr(&bars.scale_empty[i]), 8);
+            mbar_init(smem_addr(&bars.scale_empty[i]), 16);
         }
         for (int i = 0; i < kPartSlots; ++i) {
             mbar_init(smem_addr(&bars.part_full[i]), 1);
-            mbar_init(smem_addr(&bars.part_empty[i]), 15);         // every warp but the one that writes them
+            mbar_init(smem_addr(&bars.part_empty[i]), 23);         // every warp but the one that writes them
         }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) { tmem_alloc(smem_addr(&tmem_holder), 512); tmem_relinquish(); }
+    if (warp == kProductWarp) { tmem_alloc(smem_addr(&tmem_holder), 512); tmem_relinquish(); }
 
     // --- this CTA's share of the axis of key blocks
     const int per = (p.c.sequences + kPromptThreads - 1) / kPromptThreads;
@@ -433,16 +445,28 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             ++n_part;
         };
 
-        if (warp < 8) {
+        if (warp < kConvertWarp) {
             // ------------------------------------------------------------------ softmax
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-            const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
+            const int tile = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t s_tmem = tmem + tile * 128 + lanes, o_tmem = tmem + S::kO + tile * DIM + lanes;
             const int row_token = row / p.head_tile, row_head = row - row_token * p.head_tile;
-            uint32_t blocks_seen = 0, scale_uses = 0;
+            uint32_t blocks_seen = 0, scale_uses = 0, meetings = 0, o_uses = 0;
+            bool ok = true, more = true;
+            // What the other half's thread of this row says (both are there when this returns).
+            auto meet = [&](float mine) -> float {
+                const uint32_t bar = smem_addr(&bars.meet[tile][warp & 3]);
+                met[meetings & 1][tile][half][row] = mine;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+                ok = prompt_wait(bar, meetings & 1, abort, wait_code(15, tile));
+                const float other = met[meetings & 1][tile][half ^ 1][row];
+                ++meetings;
+                return other;
+            };
 
-            // This row's query to shared memory as fp16 times a power of two; returns what the scores are times.
+            // This row's query (this half of its dimensions) to shared memory as fp16 times a power of two; returns
+            // what the scores are times.
             auto load_q = [&](const PromptItem& it) -> float {
                 const int tok = it.token0 + tile * p.token_tile + row_token, hd = it.head0 + row_head;
                 const bool there = row_token < p.token_tile && tok < it.count && hd < p.a.group;
@@ -460,8 +484,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         up = __uint_as_float((uint32_t)(shift + 127) << 23) * p.sign;
                         top = (uint32_t)(127 - max(-120, min(126, shift))) << 23;
                     }
-#pragma unroll
-                    for (int c = 0; c < DIM / 8; ++c) {
+#pragma unroll 2
+                    for (int c = pass == 1 ? half * (DIM / 16) : 0; c < (pass == 1 ? (half + 1) * (DIM / 16) : DIM / 8); ++c) {
                         uint4 w = make_uint4(0, 0, 0, 0);
                         if (there && c * 8 < p.c.head_dim) {
                             if (vector) w = *reinterpret_cast<const uint4*>(q + c * 8);
@@ -510,7 +534,6 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             };
 
             float q_scale = parts[0].mine1[tile] > parts[0].mine0[tile] ? load_q(parts[0].it) : 0.0f;
-            bool ok = true, more = true;
             while (more && ok) {
                 const PromptPart& part = parts[n_part % kPartSlots];
                 const PromptItem& it = part.it;
@@ -536,41 +559,27 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     const PromptScales& sc = scales[slot];
                     const float ratio = sc.ratio;
                     unit = sc.unit;
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        ok = prompt_wait(smem_addr(&bars.s_full[tile][half]), blocks_seen & 1, abort, wait_code(2, tile));
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t s_half = s_tmem + half * kHalf;
-                        const float *key_scales = sc.key + half * 4, *weights = sc.weight + half * 4;
-                        const int key = key0 + j * kBlock + half * kHalf;
-                        const bool whole = key + kHalf <= all_hi && key >= all_lo;
-                        float s[kHalf];
-                        tmem_ld32(s_half, s);
-                        tmem_ld32(s_half + 32, s + 32);
-                        tmem_ld_wait();
-                        uint32_t seen[2] = {0, 0};
-                        if (!whole) {
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                seen[c] = prompt_seen(c * 32, lo - key, hi - key);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (!((seen[c] >> i) & 1)) s[c * 32 + i] = -INFINITY;
-                            }
-                        }
-                        float top = prompt_top(s, key_scales, q_scale);
+                    ok = prompt_wait(smem_addr(&bars.s_full[tile]), blocks_seen & 1, abort, wait_code(2, tile));
+                    if (!ok) break;
+                    ++blocks_seen;
+                    tc_fence_after();
+                    const uint32_t s_half = s_tmem + half * kHalf;
+                    const float *key_scales = sc.key + half * 4, *weights = sc.weight + half * 4;
+                    const int key = key0 + j * kBlock + half * kHalf;
+                    const bool whole = key + kHalf <= all_hi && key >= all_lo;
+                    float top = whole ? prompt_top<true>(s_half, key_scales, q_scale, 0, 0)
+                                      : prompt_top<false>(s_half, key_scales, q_scale, lo - key, hi - key);
+                    top = fmaxf(top, meet(top));
+                    if (!ok) break;
+                    if (__any_sync(0xffffffffu, top > m + kScoreLag || ratio != 1.0f)) {
                         if (!(top > m + kScoreLag)) top = m;
-                        const float keep = prompt_exp2(m - top), change = half == 0 ? keep * ratio : keep;
+                        const float keep = prompt_exp2(m - top), change = keep * ratio;
                         m = top;
-                        if (__any_sync(0xffffffffu, keep != 1.0f || change != 1.0f) && (half > 0 || j > mine0)) {
-                            // O must be at rest: the product of the half before may not be finished
-                            ok = prompt_wait(smem_addr(&bars.o_done[tile][half ^ 1]), (blocks_seen - (half ^ 1)) & 1, abort, wait_code(3, tile));
-                            if (!ok) break;
-                            tc_fence_after();
-                            l *= keep;
+                        l *= keep;
+                        // S(j) has arrived, so the product of the block before has: O is at rest
+                        if (j > mine0) {
 #pragma unroll 1
-                            for (int ch = 0; ch < DIM / 16; ++ch) {
+                            for (int ch = half * (DIM / 32); ch < (half + 1) * (DIM / 32); ++ch) {
                                 float o[16];
                                 uint32_t v[16];
                                 tmem_ld16(o_tmem + ch * 16, o);
@@ -580,16 +589,16 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                 tmem_st16(o_tmem + ch * 16, v);
                             }
                         }
-                        l += whole ? prompt_weights<true>(s, seen, s_half, key_scales, weights, q_scale, m)
-                                   : prompt_weights<false>(s, seen, s_half, key_scales, weights, q_scale, m);
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_addr(&bars.p_ready[tile][half]));
                     }
-                    if (!ok) break;
-                    ++blocks_seen;
-                    if (lane == 0) mbar_arrive(smem_addr(&bars.scale_empty[slot]));
+                    l += whole ? prompt_weights<true>(s_half, key_scales, weights, q_scale, m, 0, 0)
+                               : prompt_weights<false>(s_half, key_scales, weights, q_scale, m, lo - key, hi - key);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_addr(&bars.p_ready[tile][half]));
+                        mbar_arrive(smem_addr(&bars.scale_empty[slot]));
+                    }
                 }
                 if (!ok) break;
                 // the next part's queries before this one's output: their products can start meanwhile
@@ -605,70 +614,67 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 const bool any = mine1 > mine0;
                 if (any) {
-                    ok = prompt_wait(smem_addr(&bars.o_done[tile][0]), (blocks_seen - 1) & 1, abort, wait_code(3, tile)) &&
-                         prompt_wait(smem_addr(&bars.o_done[tile][1]), (blocks_seen - 1) & 1, abort, wait_code(3, tile));
+                    l += meet(l);
+                    ok = ok && prompt_wait(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
+                    ++o_uses;
                     if (!ok) break;
                     tc_fence_after();
                 }
-                const bool begins = part.step == 0, ends = part.stop == it.blocks;
-                if (begins && ends) {
-                    const bool there = row_token < p.token_tile && tok < it.count && it.head0 + row_head < p.a.group;
-                    const int64_t token = it.begin + tok, head = (int64_t)it.kv_head * p.a.group + it.head0 + row_head;
-                    const bool empty = m == kNoScore && l == 0.0f;
-                    const float inv = empty ? 0.0f : unit / l;
-                    uint16_t* out = static_cast<uint16_t*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride;
-                    const bool vector = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-#pragma unroll
-                    for (int ch = 0; ch < DIM / 32; ++ch) {
-                        float o[32];
-                        if (any) { tmem_ld32(o_tmem + ch * 32, o); tmem_ld_wait(); }
-                        uint32_t h[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int a = FORMAT == RNS_KV_INT8 ? (i >> 1) * 4 + (i & 1) : 2 * i;
-                            const int b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1;
-                            const float x = empty ? 0.0f : o[a] * inv, y = empty ? 0.0f : o[b] * inv;
-                            if (p.a.type == RNS_F16) {
-                                const __half2 f = __floats2half2_rn(x, y);
-                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
-                            } else {
-                                const __nv_bfloat162 f = __floats2bfloat162_rn(x, y);
-                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
-                            }
-                        }
-                        if (there) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (ch * 32 + i * 8 >= p.c.head_dim) break;
-                                if (vector) *reinterpret_cast<uint4*>(out + ch * 32 + i * 8) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-                                else {
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e) out[ch * 32 + i * 8 + e] = (uint16_t)(h[4 * i + e / 2] >> (16 * (e & 1)));
-                                }
-                            }
-                        }
+                // half of the row's output: to its place, or as a piece of it (largest score, sum, O) to the workspace
+                const bool complete = part.step == 0 && part.stop == it.blocks, empty = m == kNoScore && l == 0.0f;
+                const bool there = row_token < p.token_tile && it.token0 + tile * p.token_tile + row_token < it.count &&
+                                   it.head0 + row_head < p.a.group;
+                const int64_t token = it.begin + it.token0 + tile * p.token_tile + row_token;
+                const int64_t head = (int64_t)it.kv_head * p.a.group + it.head0 + row_head;
+                const int which = part.left == w1 - w0 ? 0 : 1;
+                float* piece = p.partial + ((int64_t)blockIdx.x * 2 + which) * S::kPartial;
+                const int at = tile * kTileRows + row;
+                const float factor = complete ? (empty ? 0.0f : unit / l) : unit;
+#pragma unroll 1
+                for (int d = half * (DIM / 2); d < (half + 1) * (DIM / 2); d += 16) {
+                    float o[16];
+                    if (any) {
+                        tmem_ld16(o_tmem + d, o);
+                        tmem_ld_wait();
                     }
-                    if (p.a.lse != nullptr && there)
-                        p.a.lse[token * p.a.heads + head] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-                } else {
-                    const int which = part.left == w1 - w0 ? 0 : 1;
-                    float* piece = p.partial + ((int64_t)blockIdx.x * 2 + which) * S::kPartial;
-                    const int at = tile * kTileRows + row;
-                    piece[at] = m;
-                    piece[2 * kTileRows + at] = l;
-                    float4* out = reinterpret_cast<float4*>(piece + 4 * kTileRows + at * DIM);
 #pragma unroll
-                    for (int ch = 0; ch < DIM / 32; ++ch) {
-                        float o[32];
-                        if (any) { tmem_ld32(o_tmem + ch * 32, o); tmem_ld_wait(); }
+                    for (int i = 0; i < 16; ++i) o[i] = any ? o[i] * factor : 0.0f;
+                    if (FORMAT == RNS_KV_INT8) {                    // columns hold dimensions 0 2 1 3 of every four
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) { const float x = o[i + 1]; o[i + 1] = o[i + 2]; o[i + 2] = x; }
+                    }
+                    if (!complete) {
+                        float4* to = reinterpret_cast<float4*>(piece + 4 * kTileRows + at * DIM + d);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    } else if (there && d < p.c.head_dim) {
+                        uint32_t h[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const int a = 4 * i, b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1, c = FORMAT == RNS_KV_INT8 ? a + 1 : a + 2;
-                            out[ch * 8 + i] = any ? make_float4(o[a] * unit, o[b] * unit, o[c] * unit, o[a + 3] * unit)
-                                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (p.a.type == RNS_F16) {
+                                const __half2 f = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
+                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
+                            } else {
+                                const __nv_bfloat162 f = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
+                            }
+                        }
+                        uint16_t* out = static_cast<uint16_t*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride + d;
+                        if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+                            reinterpret_cast<uint4*>(out)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+                            reinterpret_cast<uint4*>(out)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) out[e] = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
                         }
                     }
-                    if (begins && t == 0) {
+                }
+                if (complete) {
+                    if (p.a.lse != nullptr && there && half == 0)
+                        p.a.lse[token * p.a.heads + head] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                } else {
+                    if (half == 0) { piece[at] = m; piece[2 * kTileRows + at] = l; }
+                    if (part.step == 0 && t == 0) {
                         // this CTA holds the first piece: it names the item and where its pieces are
                         const int64_t end = w1 - part.left + it.blocks;
                         int64_t last = (end - 1) * ctas / total;
@@ -684,10 +690,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 q_scale = next_scale;
                 part_done();
             }
-        } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        }
-        if (warp >= 8 && warp < 12) {
+        } else if (warp < kProductWarp) {
             // ------------------------------------------------------------------ 8-bit tiles -> fp16 tiles
             const int lane_key = ((lane >> 3) & 3) ^ (((lane >> 2) & 1) * 5), lane_chunk = lane & 3;
             // byte of this lane's chunk in 8 keys as TMA swizzled them, and of its two chunks in a part of the fp16 tile
@@ -713,7 +716,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         // four chunks of keys k and k ^ 5, whose swizzles differ in bits 0 and 2: neither the
                         // 16-byte loads nor the stores meet a bank twice, and every swizzle is a constant of the lane.
 #pragma unroll 2
-                        for (int u = warp - 8; u < kBlock / 8 * S::kParts; u += 4) {
+                        for (int u = warp - kConvertWarp; u < kBlock / 8 * S::kParts; u += 4) {
                             const int part64 = u % S::kParts, keys = u / S::kParts * 8;
                             const uint32_t at = from + keys * DIM + raw_at + (DIM == 128 ? (part64 << 6 ^ raw_flip) : 0);
                             uint32_t w[4];
@@ -740,12 +743,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 part_done();
             }
-        } else if (warp == 12) {
+        } else if (warp == kProductWarp) {
             // ------------------------------------------------------------------ products
             // The whole warp walks along and one elected lane issues: descriptors are then uniform values,
             // which the instruction takes from uniform registers (from one lane's registers each product
             // cost over 250 cycles to issue).
-            const uint32_t idesc_s = f16_idesc(128, kHalf, false), idesc_o = f16_idesc(128, DIM, true);
+            const uint32_t idesc_s = f16_idesc(128, kBlock, false), idesc_o = f16_idesc(128, DIM, true);
             uint32_t n = 0, q_uses[2] = {0, 0}, p_uses = 0;              // p_uses: a phase bit for each tile's half
             bool ok = true, more = true;
             const auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -762,8 +765,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int from1 = uniform(part.mine0[1]), to1 = uniform(part.mine1[1]);
                 if (to0 > from0) wait(bars.q_full[0], q_uses[0]++, 6, 0);
                 if (to1 > from1) wait(bars.q_full[1], q_uses[1]++, 6, 1);
-                // Half by half: block j's second product, then block j + 1's first into the same columns, tile
-                // after tile, so that the other half's scores are there while one is exponentiated.
+                // Block j's second product, then block j + 1's first into the same columns, tile after tile.
                 // n counts tiles: keys of block j at n, its values at n + 1, the next keys at n + 2.
 #pragma unroll 1
                 for (int j = live0 - 1; j < live1 && live0 < live1; ++j) {
@@ -773,35 +775,38 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     if (now) wait(bars.full[v], (n + 1) / S::kRing, 8, v);
                     if (again) wait(bars.full[k_next], k_index / S::kRing, 7, k_next);
 #pragma unroll 1
-                    for (int step = 0; step < 4 && ok; ++step) {
-                        const int tile = step & 1, half = step >> 1;
+                    for (int tile = 0; tile < 2 && ok; ++tile) {
                         const int from = tile ? from1 : from0, to = tile ? to1 : to0;
                         if (j >= from && j < to) {
-                            wait(bars.p_ready[tile][half], p_uses >> (step * 8), 9, step);
-                            p_uses ^= 1u << (step * 8);
-                            if (!ok) break;
-                            const uint32_t d = tm + S::kO + tile * DIM, a = tm + tile * 128 + half * kHalf;
-                            const uint32_t first = j == from && half == 0 ? 0 : 1;
-                            const uint64_t b = mn_desc(ring + v * S::kTile + half * (kHalf * 128), kBlock * 128, 1024);
-                            if (elect_one()) {
+#pragma unroll 1
+                            for (int half = 0; half < 2; ++half) {
+                                const int bit = (tile * 2 + half) * 8;
+                                wait(bars.p_ready[tile][half], p_uses >> bit, 9, tile);
+                                p_uses ^= 1u << bit;
+                                if (!ok) break;
+                                const uint32_t d = tm + S::kO + tile * DIM, a = tm + tile * 128 + half * kHalf;
+                                const uint32_t first = j == from && half == 0 ? 0 : 1;
+                                const uint64_t b = mn_desc(ring + v * S::kTile + half * (kHalf * 128), kBlock * 128, 1024);
+                                if (elect_one()) {
 #pragma unroll
-                                for (int k = 0; k < kHalf / 16; ++k)
-                                    umma_f16_ts(d, a + k * 8, b + (k * 2048 >> 4), idesc_o, k > 0 ? 1 : first);
-                                umma_commit(smem_addr(&bars.o_done[tile][half]));
+                                    for (int k = 0; k < kHalf / 16; ++k)
+                                        umma_f16_ts(d, a + k * 8, b + (k * 2048 >> 4), idesc_o, k > 0 ? 1 : first);
+                                    if (half == 1 && j + 1 == to) umma_commit(smem_addr(&bars.o_full[tile]));
+                                }
+                                __syncwarp();
                             }
-                            __syncwarp();
                         }
-                        if (again && j + 1 >= from && j + 1 < to) {
-                            const uint32_t d = tm + tile * 128 + half * kHalf;
+                        if (ok && again && j + 1 >= from && j + 1 < to) {
+                            const uint32_t d = tm + tile * 128;
                             const uint64_t a = make_smem_desc(q_smem + tile * (S::kQ / 2), 128);
-                            const uint64_t b = make_smem_desc(ring + k_next * S::kTile + half * (kHalf * 128), 128);
+                            const uint64_t b = make_smem_desc(ring + k_next * S::kTile, 128);
                             if (elect_one()) {
 #pragma unroll
                                 for (int k = 0; k < DIM / 16; ++k) {
                                     const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
                                     umma_f16(d, a + off, b + off, idesc_s, k > 0);
                                 }
-                                umma_commit(smem_addr(&bars.s_full[tile][half]));
+                                umma_commit(smem_addr(&bars.s_full[tile]));
                             }
                             __syncwarp();
                         }
@@ -819,7 +824,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             // nothing may still be on its way to this CTA's barriers when it leaves
             for (uint32_t i = n > S::kRing ? n - S::kRing : 0; i < n && ok; ++i)
                 wait(bars.empty[i % S::kRing], i / S::kRing, 10, i % S::kRing);
-        } else if (warp == 13) {
+        } else if (warp == kCopyWarp) {
             // ------------------------------------------------------------------ copies
             uint32_t n = 0;
             bool ok = true, more = true;
@@ -850,7 +855,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 part_done();
             }
-        } else if (warp == 14) {
+        } else if (warp == kScaleWarp) {
             // ------------------------------------------------------------------ scales of the pages
             uint32_t n = 0;
             bool ok = true, more = true;
@@ -891,7 +896,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 part_done();
             }
-        } else if (warp == 15) {
+        } else if (warp == kPartWarp) {
             // ------------------------------------------------------------------ parts
             PromptPart part = parts[0];
             bool ok = true;
@@ -912,7 +917,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == kProductWarp) tmem_dealloc(tmem, 512);
     if (abort_word != 0 && t == 0 && p.c.status != nullptr) *p.c.status = RNS_ERR_DEVICE_TIMEOUT;
 }
 
@@ -970,7 +975,7 @@ int64_t kv_prompt_workspace(const KvView& c) {
 
 template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* workspace, cudaStream_t st) {
     using S = PromptShape<DIM>;
-    static_assert(S::kSmem + 2048 <= 227 * 1024, "one CTA per SM");
+    static_assert(S::kSmem + 6144 <= 227 * 1024, "one CTA per SM");
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
     p.box_rows = p.c.page_tokens;
@@ -984,9 +989,6 @@ template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* w
     p.meta = static_cast<int32_t*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)sms * 32);
     const auto kernel = kv_prompt_kernel<DIM, FORMAT>;
-    // the kernel's own split of the registers counts on this launch (looked up once per process)
-    static const int regs = [&] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0; }();
-    if (regs < kLaunchRegs) return fail(RNS_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, not %d", regs, kLaunchRegs);
     RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     kernel<<<sms, kPromptThreads, S::kSmem, st>>>(maps[0], maps[1], p);
     RNS_CUDA_OK(cudaGetLastError());
