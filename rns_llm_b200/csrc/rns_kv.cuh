@@ -87,15 +87,17 @@ RNS_HD KvSpan kv_span(const KvView& c, const int32_t* lens, const int32_t* start
     }
     return s;
 }
-// Page of the cache that holds page `nth` of sequence b, or -1 (status word set).
-RNS_HD int kv_page(const KvView& c, int b, int nth) {
-    const int32_t page = c.table[(int64_t)b * c.table_stride + nth];
+// Entry `nth` of sequence b's row of the page table, and the page it names: -1 (status word set) when the
+// cache has no such page.
+RNS_HD int32_t kv_entry(const KvView& c, int b, int nth) { return c.table[(int64_t)b * c.table_stride + nth]; }
+RNS_HD int kv_named(const KvView& c, int32_t page) {
     if (page < 0 || (int64_t)page >= c.pages) {
         kv_flag(c);
         return -1;
     }
     return page;
 }
+RNS_HD int kv_page(const KvView& c, int b, int nth) { return kv_named(c, kv_entry(c, b, nth)); }
 
 #ifdef __CUDACC__
 template <typename T> __device__ __forceinline__ float kv_to_float(T v);

@@ -22,21 +22,25 @@
 // * Work is cut as there: one axis of key blocks over all items, equal shares, pieces joined by a
 //   second kernel.
 //
-// Warps 0-15: softmax (four a tile and half of the block's keys: one thread for a row and half; the same
-// warps fetch the queries and store the outputs, half of the dimensions each); 16-19: conversion; 20: issues
-// the products; 21: copies; 22: scales of the pages; 23: the list of what there is to do.
+// Warps 0-3 and 4-7: softmax of a tile, a thread a row (the same warps fetch the queries and store the
+// outputs); 8-11: conversion; 12: issues the products; 13: copies; 14: scales of the pages; 15: the list of
+// what there is to do.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 
 namespace rns {
 
-constexpr int kPromptThreads = 768;
-constexpr int kConvertWarp = 16, kProductWarp = 20, kCopyWarp = 21, kScaleWarp = 22, kPartWarp = 23;
-constexpr int kBlock = 128, kHalf = 64;   // keys of a block, and of the halves that a softmax thread takes
+constexpr int kPromptThreads = 512;
+constexpr int kConvertWarp = 8, kProductWarp = 12, kCopyWarp = 13, kScaleWarp = 14, kPartWarp = 15;
+constexpr int kBlock = 128;               // keys of a block
 constexpr int kTileRows = 128;
 constexpr float kNoScore = -1.7e38f;      // below every score: "nothing seen yet"
 constexpr float kScoreLag = 8.0f;
 constexpr int kScaleSlots = 4, kPartSlots = 4;
+// Registers: a softmax thread holds its row's scores of a block.  8 warps of kSoftmaxRegs and 8 of kOtherRegs
+// must not exceed what the block was launched with, 16 warps of kLaunchRegs.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
+static_assert(8 * kSoftmaxRegs + 8 * kOtherRegs <= 16 * kLaunchRegs, "register split");
 
 struct PromptParams {
     KvView c;
@@ -142,7 +146,7 @@ template <int DIM> struct PromptShape {
     static constexpr int kParts = DIM / 64;                        // 64-dimension parts of a tile
     static constexpr int kTile = kBlock * DIM * 2;                 // fp16 tile of keys or values
     static constexpr int kRaw = kBlock * DIM;                      // the same in 8 bits
-    static constexpr int kRing = DIM == 64 ? 4 : 3, kRawRing = DIM == 64 ? 4 : 3;
+    static constexpr int kRing = DIM == 64 ? 4 : 3, kRawRing = 4;
     static constexpr int kQ = 2 * kTileRows * DIM * 2;
     static constexpr int kSmem = 1024 + kQ + kRing * kTile + kRawRing * kRaw;
     static constexpr int kPartial = 2 * kTileRows * (DIM + 2);
@@ -179,6 +183,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
           "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld8f(uint32_t taddr, float (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -241,17 +251,25 @@ __device__ __forceinline__ uint32_t half_pair_e4m3(uint32_t x) {
     return r;
 }
 
-// Waits of whole warps, bounded by about a second of SM clock.  Sixteen warps run eight different programs
-// here, and the instruction cache is what they compete for first: with waits of 64 inlined polls and rows of
-// 128 columns unrolled in two forms, "no instruction" was the largest stall by far.
+// Waits of whole warps, bounded by about a second of SM clock.  A poll may sleep for up to 0.1 ms until
+// its phase completes: most of 24 warps wait at any time, and without a time to sleep their polls took
+// more issue slots than the work.  Waits are kept small, too: eight different programs share the
+// instruction cache.
+__device__ __forceinline__ bool prompt_poll(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(100000u) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity, volatile int* abort, int where) {
     bool ok = mbar_try_wait(bar, parity);
     if (!__all_sync(0xffffffffu, ok)) {
         const uint32_t t0 = (uint32_t)clock();
 #pragma unroll 1
-        for (uint32_t spin = 1; !ok; ++spin) {
-            ok = mbar_try_wait(bar, parity);
-            if (!ok && (spin & 255u) == 0) {
+        while (!ok) {
+            ok = prompt_poll(bar, parity);
+            if (!ok) {
                 if (*abort) break;
                 if ((uint32_t)clock() - t0 > 2000000000u) {
                     if (*abort == 0) *abort = where;
@@ -265,7 +283,7 @@ __device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity, volat
 }
 
 struct PromptBars {
-    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2][2], o_full[2], q_full[2], meet[2][4];
+    uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2], o_full[2], q_full[2];
     uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots], part_full[kPartSlots], part_empty[kPartSlots];
 };
 struct PromptScales {
@@ -279,61 +297,99 @@ __device__ __forceinline__ uint32_t prompt_seen(int at, int lo, int hi) {
     const int a = min(max(lo - at, 0), 32), b = min(max(hi - at, 0), 32);
     return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
 }
-// The largest score of a row's half block, 16 columns (a page's or part of one) at a time; key: their scales.
-// WHOLE: the row sees every column, otherwise columns [lo, hi).
-template <bool WHOLE>
-__device__ __forceinline__ float prompt_top(uint32_t s_tmem, const float* key, float q_scale, int lo, int hi) {
+// The largest score of a row of a block, of which it sees every column.
+__device__ __forceinline__ float prompt_top(uint32_t s_tmem, const PromptScales& sc, float q_scale) {
+    float s[kBlock];
+#pragma unroll
+    for (int i = 0; i < kBlock; i += 32) tmem_ld32(s_tmem + i, s + i);
+    tmem_ld_wait();
     float top = kNoScore;
-#pragma unroll 1
-    for (int g = 0; g < kHalf / 16; ++g) {
-        float s[16];
-        tmem_ld16(s_tmem + g * 16, s);
-        tmem_ld_wait();
-        if (!WHOLE) {
-            const uint32_t seen = prompt_seen(g * 16, lo, hi);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!((seen >> i) & 1)) s[i] = -INFINITY;
+    for (int g = 0; g < kBlock / 16; ++g) {
+        float a = max3(s[g * 16], s[g * 16 + 1], s[g * 16 + 2]), b = max3(s[g * 16 + 3], s[g * 16 + 4], s[g * 16 + 5]);
+#pragma unroll
+        for (int i = 6; i < 14; i += 4) {
+            a = max3(a, s[g * 16 + i], s[g * 16 + i + 1]);
+            b = max3(b, s[g * 16 + i + 2], s[g * 16 + i + 3]);
         }
-        float best = fmaxf(s[0], s[15]);
-#pragma unroll
-        for (int i = 1; i < 15; i += 2) best = max3(best, s[i], s[i + 1]);
-        top = fmaxf(top, best * (key[g] * q_scale));
+        a = max3(a, s[g * 16 + 14], s[g * 16 + 15]);
+        top = fmaxf(top, fmaxf(a, b) * (sc.key[g] * q_scale));
     }
     return top;
 }
-// Scores -> weights 2^(s f - m), whose sum is returned, and times the values' scale as fp16 into the place of
-// the scores.
-template <bool WHOLE>
-__device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const float* key, const float* weights, float q_scale,
-                                                float m, int lo, int hi) {
+// Scores -> weights 2^(s f - m), whose sum is returned, and times the values' scale as fp16 into the place of the
+// scores.  A loop over 32 columns, read a second time, rather than 128 held and unrolled: the code of all
+// eight programs has to stay in the instruction caches.  The next columns are fetched as soon as the
+// multiply-adds have taken these.
+__device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const PromptScales& sc, float q_scale, float m) {
     const Pair minus_m = pair(-m, -m);
-    Pair sum = pair(0.0f, 0.0f);
+    Pair sums[4] = {0, 0, 0, 0};                                    // independent: the additions must not wait for one another
+    float s[32];
+    tmem_ld32(s_tmem, s);
 #pragma unroll 1
-    for (int g = 0; g < kHalf / 16; ++g) {
-        float s[16];
-        tmem_ld16(s_tmem + g * 16, s);
-        const float f = key[g] * q_scale, weight = weights[g];
-        const uint32_t seen = WHOLE ? 0 : prompt_seen(g * 16, lo, hi);
-        uint32_t w[8];
+    for (int ch = 0; ch < 4; ++ch) {
+        Pair e[16];
+        const float f0 = sc.key[ch * 2] * q_scale, f1 = sc.key[ch * 2 + 1] * q_scale;
+        const float w0 = sc.weight[ch * 2], w1 = sc.weight[ch * 2 + 1];
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const Pair x = fma2(pair(s[2 * i], s[2 * i + 1]), pair(f, f), minus_m);
-            Pair e = pair(prompt_exp2(pair_x(x)), prompt_exp2(pair_y(x)));
-            Pair pw = mul2(e, pair(weight, weight));
-            if (!WHOLE) {                                           // not NaN from a scale that this row does not see
-                const bool a = (seen >> (2 * i)) & 1, b = (seen >> (2 * i + 1)) & 1;
-                e = pair(a ? pair_x(e) : 0.0f, b ? pair_y(e) : 0.0f);
-                pw = pair(a ? pair_x(pw) : 0.0f, b ? pair_y(pw) : 0.0f);
-            }
-            sum = add2(sum, e);
+        for (int i = 0; i < 16; ++i)
+            e[i] = fma2(pair(s[2 * i], s[2 * i + 1]), i < 8 ? pair(f0, f0) : pair(f1, f1), minus_m);
+        tmem_ld32(s_tmem + (ch < 3 ? ch + 1 : 3) * 32, s);          // (the last time to no purpose: its columns are not written yet)
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            e[i] = pair(prompt_exp2(pair_x(e[i])), prompt_exp2(pair_y(e[i])));
+            sums[i & 3] = add2(sums[i & 3], e[i]);
+            const Pair pw = mul2(e[i], i < 8 ? pair(w0, w0) : pair(w1, w1));
             const __half2 h = __floats2half2_rn(pair_x(pw), pair_y(pw));
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
+        tmem_st16(s_tmem + ch * 16, w);
+    }
+    tmem_ld_wait();
+    const Pair sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+    return pair_x(sum) + pair_y(sum);
+}
+// The same for rows that see columns [lo, hi) only: at the diagonal, a window's edge or a sequence's end.  16
+// columns at a time from tensor memory, to keep the code small.
+__device__ __forceinline__ float prompt_top_seen(uint32_t s_tmem, const PromptScales& sc, float q_scale, int lo, int hi) {
+    float top = kNoScore;
+#pragma unroll 1
+    for (int g = 0; g < kBlock / 16; ++g) {
+        float s[16];
+        tmem_ld16(s_tmem + g * 16, s);
+        tmem_ld_wait();
+        const uint32_t seen = prompt_seen(g * 16, lo, hi);
+        float best = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) best = fmaxf(best, (seen >> i) & 1 ? s[i] : -INFINITY);
+        top = fmaxf(top, best * (sc.key[g] * q_scale));
+    }
+    return top;
+}
+__device__ __forceinline__ float prompt_weights_seen(uint32_t s_tmem, const PromptScales& sc, float q_scale, float m, int lo, int hi) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int g = 0; g < kBlock / 16; ++g) {
+        float s[16];
+        tmem_ld16(s_tmem + g * 16, s);
+        tmem_ld_wait();
+        const uint32_t seen = prompt_seen(g * 16, lo, hi);
+        const float f = sc.key[g] * q_scale, weight = sc.weight[g];
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            // zero where the row does not see, not NaN from a scale that it does not see
+            const bool a = (seen >> i) & 1, b = (seen >> (i + 1)) & 1;
+            const float e0 = a ? prompt_exp2(fmaf(s[i], f, -m)) : 0.0f, e1 = b ? prompt_exp2(fmaf(s[i + 1], f, -m)) : 0.0f;
+            sum += e0 + e1;
+            const __half2 h = __floats2half2_rn(a ? e0 * weight : 0.0f, b ? e1 * weight : 0.0f);
+            w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+        }
         tmem_st8(s_tmem + g * 8, w);
     }
-    return pair_x(sum) + pair_y(sum);
+    return sum;
 }
 
 template <int DIM, int FORMAT>
@@ -348,7 +404,6 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __shared__ __align__(16) PromptScales scales[kScaleSlots];
     __shared__ int64_t scan[kPromptThreads / 32];
     __shared__ PromptPart parts[kPartSlots];
-    __shared__ float met[2][2][2][kTileRows];                      // [turn][tile][half][row]
     __shared__ int abort_word;
     __shared__ uint32_t tmem_holder;
 
@@ -363,17 +418,16 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_addr(&bars.s_full[i]), 1);
             mbar_init(smem_addr(&bars.o_full[i]), 1);
-            for (int h = 0; h < 2; ++h) mbar_init(smem_addr(&bars.p_ready[i][h]), 4);
-            for (int h = 0; h < 4; ++h) mbar_init(smem_addr(&bars.meet[i][h]), 2);
-            mbar_init(smem_addr(&bars.q_full[i]), 8);
+            mbar_init(smem_addr(&bars.p_ready[i]), 4);
+            mbar_init(smem_addr(&bars.q_full[i]), 4);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
             mbar_init(smem_addr(&bars.scale_full[i]), 1);
-            mbar_init(smem_addr(&bars.scale_empty[i]), 16);
+            mbar_init(smem_addr(&bars.scale_empty[i]), 8);
         }
         for (int i = 0; i < kPartSlots; ++i) {
             mbar_init(smem_addr(&bars.part_full[i]), 1);
-            mbar_init(smem_addr(&bars.part_empty[i]), 23);         // every warp but the one that writes them
+            mbar_init(smem_addr(&bars.part_empty[i]), 15);         // every warp but the one that writes them
         }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -447,26 +501,15 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
         if (warp < kConvertWarp) {
             // ------------------------------------------------------------------ softmax
-            const int tile = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+            const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t s_tmem = tmem + tile * 128 + lanes, o_tmem = tmem + S::kO + tile * DIM + lanes;
             const int row_token = row / p.head_tile, row_head = row - row_token * p.head_tile;
-            uint32_t blocks_seen = 0, scale_uses = 0, meetings = 0, o_uses = 0;
+            uint32_t blocks_seen = 0, scale_uses = 0, o_uses = 0;
             bool ok = true, more = true;
-            // What the other half's thread of this row says (both are there when this returns).
-            auto meet = [&](float mine) -> float {
-                const uint32_t bar = smem_addr(&bars.meet[tile][warp & 3]);
-                met[meetings & 1][tile][half][row] = mine;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar);
-                ok = prompt_wait(bar, meetings & 1, abort, wait_code(15, tile));
-                const float other = met[meetings & 1][tile][half ^ 1][row];
-                ++meetings;
-                return other;
-            };
 
-            // This row's query (this half of its dimensions) to shared memory as fp16 times a power of two; returns
-            // what the scores are times.
+            // This row's query to shared memory as fp16 times a power of two; returns what the scores are times.
             auto load_q = [&](const PromptItem& it) -> float {
                 const int tok = it.token0 + tile * p.token_tile + row_token, hd = it.head0 + row_head;
                 const bool there = row_token < p.token_tile && tok < it.count && hd < p.a.group;
@@ -485,7 +528,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         top = (uint32_t)(127 - max(-120, min(126, shift))) << 23;
                     }
 #pragma unroll 2
-                    for (int c = pass == 1 ? half * (DIM / 16) : 0; c < (pass == 1 ? (half + 1) * (DIM / 16) : DIM / 8); ++c) {
+                    for (int c = 0; c < DIM / 8; ++c) {
                         uint4 w = make_uint4(0, 0, 0, 0);
                         if (there && c * 8 < p.c.head_dim) {
                             if (vector) w = *reinterpret_cast<const uint4*>(q + c * 8);
@@ -563,14 +606,9 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     if (!ok) break;
                     ++blocks_seen;
                     tc_fence_after();
-                    const uint32_t s_half = s_tmem + half * kHalf;
-                    const float *key_scales = sc.key + half * 4, *weights = sc.weight + half * 4;
-                    const int key = key0 + j * kBlock + half * kHalf;
-                    const bool whole = key + kHalf <= all_hi && key >= all_lo;
-                    float top = whole ? prompt_top<true>(s_half, key_scales, q_scale, 0, 0)
-                                      : prompt_top<false>(s_half, key_scales, q_scale, lo - key, hi - key);
-                    top = fmaxf(top, meet(top));
-                    if (!ok) break;
+                    const int key = key0 + j * kBlock;
+                    const bool whole = key + kBlock <= all_hi && key >= all_lo;
+                    float top = whole ? prompt_top(s_tmem, sc, q_scale) : prompt_top_seen(s_tmem, sc, q_scale, lo - key, hi - key);
                     if (__any_sync(0xffffffffu, top > m + kScoreLag || ratio != 1.0f)) {
                         if (!(top > m + kScoreLag)) top = m;
                         const float keep = prompt_exp2(m - top), change = keep * ratio;
@@ -579,24 +617,23 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         // S(j) has arrived, so the product of the block before has: O is at rest
                         if (j > mine0) {
 #pragma unroll 1
-                            for (int ch = half * (DIM / 32); ch < (half + 1) * (DIM / 32); ++ch) {
-                                float o[16];
-                                uint32_t v[16];
-                                tmem_ld16(o_tmem + ch * 16, o);
+                            for (int ch = 0; ch < DIM / 8; ++ch) {
+                                float o[8];
+                                uint32_t v[8];
+                                tmem_ld8f(o_tmem + ch * 8, o);
                                 tmem_ld_wait();
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[i] * change);
-                                tmem_st16(o_tmem + ch * 16, v);
+                                for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[i] * change);
+                                tmem_st8(o_tmem + ch * 8, v);
                             }
                         }
                     }
-                    l += whole ? prompt_weights<true>(s_half, key_scales, weights, q_scale, m, 0, 0)
-                               : prompt_weights<false>(s_half, key_scales, weights, q_scale, m, lo - key, hi - key);
+                    l += whole ? prompt_weights(s_tmem, sc, q_scale, m) : prompt_weights_seen(s_tmem, sc, q_scale, m, lo - key, hi - key);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(smem_addr(&bars.p_ready[tile][half]));
+                        mbar_arrive(smem_addr(&bars.p_ready[tile]));
                         mbar_arrive(smem_addr(&bars.scale_empty[slot]));
                     }
                 }
@@ -614,13 +651,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 const bool any = mine1 > mine0;
                 if (any) {
-                    l += meet(l);
-                    ok = ok && prompt_wait(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
+                    ok = prompt_wait(smem_addr(&bars.o_full[tile]), o_uses & 1, abort, wait_code(3, tile));
                     ++o_uses;
                     if (!ok) break;
                     tc_fence_after();
                 }
-                // half of the row's output: to its place, or as a piece of it (largest score, sum, O) to the workspace
+                // the row's output: to its place, or as a piece of it (largest score, sum, O) to the workspace
                 const bool complete = part.step == 0 && part.stop == it.blocks, empty = m == kNoScore && l == 0.0f;
                 const bool there = row_token < p.token_tile && it.token0 + tile * p.token_tile + row_token < it.count &&
                                    it.head0 + row_head < p.a.group;
@@ -631,7 +667,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int at = tile * kTileRows + row;
                 const float factor = complete ? (empty ? 0.0f : unit / l) : unit;
 #pragma unroll 1
-                for (int d = half * (DIM / 2); d < (half + 1) * (DIM / 2); d += 16) {
+                for (int d = 0; d < DIM; d += 16) {
                     float o[16];
                     if (any) {
                         tmem_ld16(o_tmem + d, o);
@@ -670,10 +706,11 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     }
                 }
                 if (complete) {
-                    if (p.a.lse != nullptr && there && half == 0)
+                    if (p.a.lse != nullptr && there)
                         p.a.lse[token * p.a.heads + head] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                 } else {
-                    if (half == 0) { piece[at] = m; piece[2 * kTileRows + at] = l; }
+                    piece[at] = m;
+                    piece[2 * kTileRows + at] = l;
                     if (part.step == 0 && t == 0) {
                         // this CTA holds the first piece: it names the item and where its pieces are
                         const int64_t end = w1 - part.left + it.blocks;
@@ -690,7 +727,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 q_scale = next_scale;
                 part_done();
             }
-        } else if (warp < kProductWarp) {
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        }
+        if (warp >= kConvertWarp && warp < kProductWarp) {
             // ------------------------------------------------------------------ 8-bit tiles -> fp16 tiles
             const int lane_key = ((lane >> 3) & 3) ^ (((lane >> 2) & 1) * 5), lane_chunk = lane & 3;
             // byte of this lane's chunk in 8 keys as TMA swizzled them, and of its two chunks in a part of the fp16 tile
@@ -749,7 +789,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             // which the instruction takes from uniform registers (from one lane's registers each product
             // cost over 250 cycles to issue).
             const uint32_t idesc_s = f16_idesc(128, kBlock, false), idesc_o = f16_idesc(128, DIM, true);
-            uint32_t n = 0, q_uses[2] = {0, 0}, p_uses = 0;              // p_uses: a phase bit for each tile's half
+            uint32_t n = 0, q_uses[2] = {0, 0}, p_uses = 0;              // p_uses: a phase bit for each tile
             bool ok = true, more = true;
             const auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
             const uint32_t tm = uniform(tmem);
@@ -767,56 +807,50 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 if (to1 > from1) wait(bars.q_full[1], q_uses[1]++, 6, 1);
                 // Block j's second product, then block j + 1's first into the same columns, tile after tile.
                 // n counts tiles: keys of block j at n, its values at n + 1, the next keys at n + 2.
+                const uint64_t q0 = make_smem_desc(q_smem, 128);
 #pragma unroll 1
                 for (int j = live0 - 1; j < live1 && live0 < live1; ++j) {
-                    const uint32_t v = (n + 1) % S::kRing;
                     const bool now = j >= live0, again = j + 1 < live1;
-                    const uint32_t k_index = now ? n + 2 : n, k_next = k_index % S::kRing;
-                    if (now) wait(bars.full[v], (n + 1) / S::kRing, 8, v);
-                    if (again) wait(bars.full[k_next], k_index / S::kRing, 7, k_next);
+                    const uint32_t k_index = now ? n + 2 : n, k_slot = k_index % S::kRing, v_slot = (n + 1) % S::kRing;
+                    // tiles are converted in order: the next keys are there after these values
+                    if (again) wait(bars.full[k_slot], k_index / S::kRing, 7, k_slot);
+                    else wait(bars.full[v_slot], (n + 1) / S::kRing, 8, v_slot);
+                    const uint64_t k_desc = make_smem_desc(ring + k_slot * S::kTile, 128);
+                    const uint64_t v_desc = mn_desc(ring + v_slot * S::kTile, kBlock * 128, 1024);
 #pragma unroll 1
                     for (int tile = 0; tile < 2 && ok; ++tile) {
                         const int from = tile ? from1 : from0, to = tile ? to1 : to0;
-                        if (j >= from && j < to) {
-#pragma unroll 1
-                            for (int half = 0; half < 2; ++half) {
-                                const int bit = (tile * 2 + half) * 8;
-                                wait(bars.p_ready[tile][half], p_uses >> bit, 9, tile);
-                                p_uses ^= 1u << bit;
-                                if (!ok) break;
-                                const uint32_t d = tm + S::kO + tile * DIM, a = tm + tile * 128 + half * kHalf;
-                                const uint32_t first = j == from && half == 0 ? 0 : 1;
-                                const uint64_t b = mn_desc(ring + v * S::kTile + half * (kHalf * 128), kBlock * 128, 1024);
-                                if (elect_one()) {
-#pragma unroll
-                                    for (int k = 0; k < kHalf / 16; ++k)
-                                        umma_f16_ts(d, a + k * 8, b + (k * 2048 >> 4), idesc_o, k > 0 ? 1 : first);
-                                    if (half == 1 && j + 1 == to) umma_commit(smem_addr(&bars.o_full[tile]));
-                                }
-                                __syncwarp();
-                            }
+                        const bool second = j >= from && j < to, first = again && j + 1 >= from && j + 1 < to;
+                        if (second) {
+                            wait(bars.p_ready[tile], p_uses >> (tile * 8), 9, tile);
+                            p_uses ^= 1u << (tile * 8);
+                            if (!ok) break;
                         }
-                        if (ok && again && j + 1 >= from && j + 1 < to) {
-                            const uint32_t d = tm + tile * 128;
-                            const uint64_t a = make_smem_desc(q_smem + tile * (S::kQ / 2), 128);
-                            const uint64_t b = make_smem_desc(ring + k_next * S::kTile, 128);
-                            if (elect_one()) {
+                        const uint32_t s_d = tm + tile * 128, o_d = tm + S::kO + tile * DIM;
+                        const uint64_t q_desc = q0 + tile * (S::kQ / 2 >> 4);
+                        if (elect_one()) {
+                            if (second) {
+#pragma unroll
+                                for (int k = 0; k < kBlock / 16; ++k)
+                                    umma_f16_ts(o_d, s_d + k * 8, v_desc + (k * 2048 >> 4), idesc_o, k > 0 || j > from);
+                                if (j + 1 == to) umma_commit(smem_addr(&bars.o_full[tile]));
+                            }
+                            if (first) {
 #pragma unroll
                                 for (int k = 0; k < DIM / 16; ++k) {
                                     const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                                    umma_f16(d, a + off, b + off, idesc_s, k > 0);
+                                    umma_f16(s_d, q_desc + off, k_desc + off, idesc_s, k > 0);
                                 }
                                 umma_commit(smem_addr(&bars.s_full[tile]));
                             }
-                            __syncwarp();
+                            if (tile == 1) {
+                                if (now) umma_commit(smem_addr(&bars.empty[v_slot]));
+                                if (again) umma_commit(smem_addr(&bars.empty[k_slot]));
+                            }
                         }
+                        __syncwarp();
                     }
                     if (!ok) break;
-                    if (elect_one()) {
-                        if (now) umma_commit(smem_addr(&bars.empty[v]));
-                        if (again) umma_commit(smem_addr(&bars.empty[k_next]));
-                    }
-                    __syncwarp();
                     if (now) n += 2;
                 }
                 if (ok) part_done();
@@ -833,23 +867,33 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const PromptPart& part = parts[n_part % kPartSlots];
                 more = !part.last;
                 const int live1 = part.live1, b = part.it.b, kv_head = part.it.kv_head, key0 = part.it.key0, length = part.it.length;
-                for (int j = part.live0; j < live1 && ok; ++j) {
-                    const int key = key0 + j * kBlock + lane * p.box_rows;
+                // Page indices of four blocks at a time, eight lanes a block, and those of the next four while
+                // these are copied: one after the other, their latency was most of a block's time.
+                const int live0 = part.live0, box = lane & 7;
+                const auto entry = [&](int at) {
+                    const int key = key0 + (at + (lane >> 3)) * kBlock + box * p.box_rows;
+                    return at + (lane >> 3) < live1 && box < boxes && key < length ? kv_entry(p.c, b, key >> p.c.page_shift) : -1;
+                };
+                int32_t next = entry(live0);
+                for (int j0 = live0; j0 < live1 && ok; j0 += 4) {
+                    const int32_t named = next;
+                    next = entry(j0 + 4);
+                    const int key = key0 + (j0 + (lane >> 3)) * kBlock + box * p.box_rows;
                     int z = (int)p.c.pages;                            // behind the last page: zeros
-                    if (lane < boxes && key < length) {
-                        const int page = kv_page(p.c, b, key >> p.c.page_shift);
+                    if (j0 + (lane >> 3) < live1 && box < boxes && key < length) {
+                        const int page = kv_named(p.c, named);
                         if (page >= 0) z = page;
                     }
 #pragma unroll 1
-                    for (int side = 0; side < 2; ++side, ++n) {
-                        const int rs = n % S::kRawRing;
+                    for (int u = 0; u < 8 && j0 + (u >> 1) < live1; ++u, ++n) {
+                        const int rs = n % S::kRawRing, side = u & 1;
                         ok = prompt_wait(smem_addr(&bars.raw_empty[rs]), ((n / S::kRawRing) & 1) ^ 1, abort, wait_code(11, rs));
                         if (!ok) break;
                         const uint32_t bar = smem_addr(&bars.raw_full[rs]);
                         if (lane == 0) mbar_arrive_expect_tx(bar, S::kRaw);
                         __syncwarp();
-                        if (lane < boxes)
-                            tma_load_3d(raw + rs * S::kRaw + lane * p.box_rows * DIM, side ? &map_v : &map_k, bar, 0,
+                        if ((lane >> 3) == (u >> 1) && box < boxes)
+                            tma_load_3d(raw + rs * S::kRaw + box * p.box_rows * DIM, side ? &map_v : &map_k, bar, 0,
                                         kv_head * p.c.page_tokens + (key & (p.c.page_tokens - 1)), z);
                     }
                 }
@@ -865,34 +909,47 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int live1 = part.live1, b = part.it.b, kv_head = part.it.kv_head, key0 = part.it.key0;
                 const int length = part.it.length, low = part.it.low;
                 float unit = 0x1p-123f;
-                for (int j = part.live0; j < live1 && ok; ++j) {
-                    const int key = key0 + j * kBlock + (lane & 7) * 16;
+                // four blocks at a time, as the copies: a lane for 16 keys
+                const int live0 = part.live0, mine = lane >> 3;
+                const auto entry = [&](int at) {
+                    const int key = key0 + (at + mine) * kBlock + (lane & 7) * 16;
+                    return at + mine < live1 && key < length ? kv_entry(p.c, b, key >> p.c.page_shift) : -1;
+                };
+                int32_t next = entry(live0);
+                for (int j0 = live0; j0 < live1 && ok; j0 += 4) {
+                    const int32_t named = next;
+                    const int key = key0 + (j0 + mine) * kBlock + (lane & 7) * 16;
                     float ks = 0.0f, vs = 0.0f;
-                    if (key < length) {
-                        const int page = kv_page(p.c, b, key >> p.c.page_shift);
+                    if (j0 + mine < live1 && key < length) {
+                        const int page = kv_named(p.c, named);
                         if (page >= 0) {
                             const int64_t block = (int64_t)page * p.c.kv_heads + kv_head;
                             ks = p.c.scale[0][block];
                             vs = p.c.scale[1][block];
                         }
                     }
+                    next = entry(j0 + 4);
                     if (!(fabsf(vs) <= 3.0e38f)) vs = __uint_as_float(0x7fc00000u);
                     // the largest of the finite ones that some row sees
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, vs == vs && key + 16 > low ? __float_as_uint(fabsf(vs)) : 0u);
-                    float ratio = 1.0f;
-                    if (__uint_as_float(top) > 16.0f * unit) {
-                        const float grown = __uint_as_float(top & 0x7f800000u);
-                        ratio = unit / grown;
-                        unit = grown;
+                    const uint32_t size = vs == vs && key + 16 > low ? __float_as_uint(fabsf(vs)) : 0u;
+#pragma unroll 1
+                    for (int i = 0; i < 4 && j0 + i < live1; ++i) {
+                        const uint32_t top = __reduce_max_sync(0xffffffffu, mine == i ? size : 0u);
+                        float ratio = 1.0f;
+                        if (__uint_as_float(top) > 16.0f * unit) {
+                            const float grown = __uint_as_float(top & 0x7f800000u);
+                            ratio = unit / grown;
+                            unit = grown;
+                        }
+                        const int slot = n % kScaleSlots;
+                        ok = prompt_wait(smem_addr(&bars.scale_empty[slot]), ((n / kScaleSlots) & 1) ^ 1, abort, wait_code(12, slot));
+                        if (!ok) break;
+                        ++n;
+                        if (mine == i) { scales[slot].key[lane & 7] = ks; scales[slot].weight[lane & 7] = vs / unit; }
+                        if (lane == 0) { scales[slot].unit = unit; scales[slot].ratio = ratio; }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_addr(&bars.scale_full[slot]));
                     }
-                    const int slot = n % kScaleSlots;
-                    ok = prompt_wait(smem_addr(&bars.scale_empty[slot]), ((n / kScaleSlots) & 1) ^ 1, abort, wait_code(12, slot));
-                    if (!ok) break;
-                    ++n;
-                    if (lane < 8) { scales[slot].key[lane] = ks; scales[slot].weight[lane] = vs / unit; }
-                    if (lane == 0) { scales[slot].unit = unit; scales[slot].ratio = ratio; }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_addr(&bars.scale_full[slot]));
                 }
                 part_done();
             }
@@ -975,7 +1032,7 @@ int64_t kv_prompt_workspace(const KvView& c) {
 
 template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* workspace, cudaStream_t st) {
     using S = PromptShape<DIM>;
-    static_assert(S::kSmem + 6144 <= 227 * 1024, "one CTA per SM");
+    static_assert(S::kSmem + 2048 <= 227 * 1024, "one CTA per SM");
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
     p.box_rows = p.c.page_tokens;
@@ -989,6 +1046,9 @@ template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* w
     p.meta = static_cast<int32_t*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)sms * 32);
     const auto kernel = kv_prompt_kernel<DIM, FORMAT>;
+    // the kernel's own split of the registers counts on this launch (looked up once per process)
+    static const int regs = [&] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0; }();
+    if (regs < kLaunchRegs) return fail(RNS_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, not %d", regs, kLaunchRegs);
     RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     kernel<<<sms, kPromptThreads, S::kSmem, st>>>(maps[0], maps[1], p);
     RNS_CUDA_OK(cudaGetLastError());
