@@ -516,64 +516,60 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int64_t at = (it.begin + tok) * p.a.q_token_stride + ((int64_t)it.kv_head * p.a.group + hd) * p.a.q_head_stride;
                 const uint16_t* q = static_cast<const uint16_t*>(p.a.q) + at;
                 const bool vector = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-                uint32_t top = 0;
-                // two passes over the row (the second from L1): its largest magnitude, then the values
-#pragma unroll 1
-                for (int pass = 0; pass < 2; ++pass) {
-                    float up = 1.0f;
-                    if (pass == 1) {
-                        const int e = (int)(top >> 23);
-                        const int shift = top == 0 || e == 255 ? 0 : max(-126, min(120, 134 - e));
-                        up = __uint_as_float((uint32_t)(shift + 127) << 23) * p.sign;
-                        top = (uint32_t)(127 - max(-120, min(126, shift))) << 23;
-                    }
-#pragma unroll 2
-                    for (int c = 0; c < DIM / 8; ++c) {
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (there && c * 8 < p.c.head_dim) {
-                            if (vector) w = *reinterpret_cast<const uint4*>(q + c * 8);
-                            else {
-                                uint16_t e[8];
+                // the whole row at once: its latency, not its bytes, is what counts between two parts
+                uint32_t w[DIM / 2];
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) e[i] = q[c * 8 + i];
-                                w = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                                               e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-                            }
-                        }
-                        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-                        float v[8];
+                for (int c = 0; c < DIM / 8; ++c) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (there && vector && c * 8 < p.c.head_dim) x = *reinterpret_cast<const uint4*>(q + c * 8);
+                    w[c * 4] = x.x; w[c * 4 + 1] = x.y; w[c * 4 + 2] = x.z; w[c * 4 + 3] = x.w;
+                }
+                if (there && !vector) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (p.a.type == RNS_F16) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&in[i]));
-                                v[2 * i] = f.x; v[2 * i + 1] = f.y;
-                            } else {
-                                v[2 * i] = __uint_as_float(in[i] << 16); v[2 * i + 1] = __uint_as_float(in[i] & 0xffff0000u);
-                            }
-                        }
-                        if (pass == 0) {
+                    for (int i = 0; i < DIM / 2; ++i)
+                        if (2 * i < p.c.head_dim) w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+                }
+                // magnitudes order like their bits in either type
+                uint32_t size = 0;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(fabsf(v[i])));
+                for (int i = 0; i < DIM / 2; ++i) size = max(size, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                const float largest = p.a.type == RNS_F16 ? __half2float(__ushort_as_half((uint16_t)size))
+                                                          : __uint_as_float(size << 16);
+                const uint32_t bits = __float_as_uint(largest);
+                const int e = (int)(bits >> 23);
+                const int shift = bits == 0 || e == 255 ? 0 : max(-126, min(120, 134 - e));
+                const float up = __uint_as_float((uint32_t)(shift + 127) << 23) * p.sign;
+                const float down = __uint_as_float((uint32_t)(127 - max(-120, min(126, shift))) << 23);
+#pragma unroll
+                for (int c = 0; c < DIM / 8; ++c) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t x = w[c * 4 + i];
+                        if (p.a.type == RNS_F16) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+                            v[2 * i] = f.x; v[2 * i + 1] = f.y;
                         } else {
-                            uint32_t h[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // int8 tiles hold dimensions 0 2 1 3 of every four
-                                const int a = FORMAT == RNS_KV_INT8 ? (i >> 1) * 4 + (i & 1) : 2 * i;
-                                const int b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1;
-                                const __half2 f = __floats2half2_rn(v[a] * up, v[b] * up);
-                                h[i] = *reinterpret_cast<const uint32_t*>(&f);
-                            }
-                            const uint32_t to = q_smem + tile * (S::kQ / 2) + (c >> 3) * (kTileRows * 128) + row * 128 +
-                                                (((c & 7) ^ (row & 7)) << 4);
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                            v[2 * i] = __uint_as_float(x << 16); v[2 * i + 1] = __uint_as_float(x & 0xffff0000u);
                         }
                     }
+                    uint32_t h[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // int8 tiles hold dimensions 0 2 1 3 of every four
+                        const int a = FORMAT == RNS_KV_INT8 ? (i >> 1) * 4 + (i & 1) : 2 * i;
+                        const int b = FORMAT == RNS_KV_INT8 ? a + 2 : a + 1;
+                        const __half2 f = __floats2half2_rn(v[a] * up, v[b] * up);
+                        h[i] = *reinterpret_cast<const uint32_t*>(&f);
+                    }
+                    const uint32_t to = q_smem + tile * (S::kQ / 2) + (c >> 3) * (kTileRows * 128) + row * 128 +
+                                        (((c & 7) ^ (row & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&bars.q_full[tile]));
-                return p.a.scale_log2 * p.sign * __uint_as_float(top);
+                return p.a.scale_log2 * p.sign * down;
             };
 
             float q_scale = parts[0].mine1[tile] > parts[0].mine0[tile] ? load_q(parts[0].it) : 0.0f;
