@@ -33,6 +33,7 @@
 namespace rns {
 
 constexpr int kDecodeWarps = 4;
+constexpr int kDecodeMostCtas = 3;      // of an SM
 constexpr int kDecodeThreads = kDecodeWarps * 32;
 constexpr float kNoMax = -1.7e38f;      // below every score: "nothing seen yet"
 constexpr float kLag = 8.0f;            // how far a score may exceed the running maximum (log2)
@@ -167,7 +168,8 @@ template <int DIM, int NT> struct DecodeShape {
     static constexpr int kKeys = DIM == 256 ? 16 : 32;             // keys of a warp's stage
     static constexpr int kStep = kKeys * kDecodeWarps;
     static constexpr int kHalf = kKeys * DIM;                      // bytes of one side of a stage
-    static constexpr int kStages = DIM == 64 ? (NT == 4 ? 5 : 6) : (NT == 4 || DIM * NT > 256) ? 2 : 3;
+    static constexpr int kCtas = DIM * NT <= 128 ? 3 : 2;          // CTAs of an SM
+    static constexpr int kStages = kCtas == 3 ? (DIM == 64 ? 4 : 2) : DIM == 64 ? (NT == 4 ? 5 : 6) : (NT == 4 || DIM * NT > 256) ? 2 : 3;
     static constexpr int kRing = kDecodeWarps * kStages * 2 * kHalf;
     static constexpr int kStride = DIM + 4;                        // floats between rows of the merge buffer
     static constexpr int kQ = kRows * (DIM + 8) * 2;               // fp16 rows of the tile
@@ -178,7 +180,7 @@ template <int DIM, int NT> struct DecodeShape {
 };
 
 template <int DIM, int NT, int FORMAT>
-__global__ void __launch_bounds__(kDecodeThreads, 2)
+__global__ void __launch_bounds__(kDecodeThreads, DecodeShape<DIM, NT>::kCtas)
 kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ DecodeParams p, int box_rows) {
     using S = DecodeShape<DIM, NT>;
@@ -396,7 +398,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 if (alive) { parity ^= 1u << slot; flying &= ~(1u << slot); }
                 const uint32_t k_base = ring + slot * 2 * S::kHalf, v_base = k_base + S::kHalf;
                 if (alive) {
-#pragma unroll
+#pragma unroll 1
                     for (int half = 0; half < KEYS / 16; ++half) {
                         const int k0 = key + half * 16;
                         if (k0 >= it.last) break;
@@ -632,19 +634,35 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ De
     const KvSpan s = kv_span(p.c, p.a.lens, p.a.starts, p.a.tokens, meta[3]);
     const int tok = tile / p.head_tiles * p.token_tile + row / p.head_tile, hd = tile % p.head_tiles * p.head_tile + row % p.head_tile;
     if (tok >= s.count || hd >= p.a.group || row >= p.token_tile * p.head_tile) return;
+    // piece 0 lies in this CTA's slot, piece i in slot 0 of the i-th CTA after it
     const float* first = p.partial + ((int64_t)blockIdx.x * 2 + slot) * S::kPartial;
-    const float* next = p.partial + ((int64_t)blockIdx.x + 1) * 2 * S::kPartial;
-    float top = first[row];
-    for (int i = 1; i < pieces; ++i) top = fmaxf(top, next[(int64_t)(i - 1) * 2 * S::kPartial + row]);
-    float sum = 0.0f, o[DIM > 128 ? 2 : 1] = {};
-    for (int i = 0; i < pieces; ++i) {
-        const float* part = i == 0 ? first : next + (int64_t)(i - 1) * 2 * S::kPartial;
-        const float f = exp2_approx(part[row] - top);
-        sum = fmaf(part[S::kRows + row], f, sum);
+    const float* next = p.partial + (int64_t)blockIdx.x * 2 * S::kPartial;
+    const auto piece = [&](int i) { return i == 0 ? first : next + (int64_t)i * 2 * S::kPartial; };
+    __shared__ float factors[128], tops[4];
+    const int t = threadIdx.x;
+    float top = kNoMax;
+    for (int i = t; i < pieces; i += 128) top = fmaxf(top, piece(i)[row]);
 #pragma unroll
-        for (int j = 0; j < (DIM > 128 ? 2 : 1); ++j) {
-            const int d = threadIdx.x + j * 128;
-            if (d < p.c.head_dim) o[j] = fmaf(part[2 * S::kRows + row * DIM + d], f, o[j]);
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    if ((t & 31) == 0) tops[t >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    float sum = 0.0f, o[DIM > 128 ? 2 : 1] = {};
+    for (int base = 0; base < pieces; base += 128) {               // pieces in key order, their loads in flight together
+        const int n = min(128, pieces - base);
+        __syncthreads();
+        if (t < n) factors[t] = exp2_approx(piece(base + t)[row] - top);
+        __syncthreads();
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float* part = piece(base + i);
+            const float f = factors[i];
+            sum = fmaf(part[S::kRows + row], f, sum);
+#pragma unroll
+            for (int j = 0; j < (DIM > 128 ? 2 : 1); ++j) {
+                const int d = min(t + j * 128, DIM - 1);
+                o[j] = fmaf(part[2 * S::kRows + row * DIM + d], f, o[j]);
+            }
         }
     }
     const float inv = top == kNoMax && sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -685,13 +703,13 @@ int64_t kv_decode_workspace(const KvView& c, const KvQuery& a, int max_new) {
     int sms = 0;
     if (sm_count(&sms) != RNS_OK) return -RNS_ERR_CUDA;
     const int64_t rows = 8 * decode_nt(c, a, max_new);
-    return (int64_t)2 * sms * (2 * rows * (decode_dim(c) + 2) * 4 + 32);
+    return (int64_t)kDecodeMostCtas * sms * (2 * rows * (decode_dim(c) + 2) * 4 + 32);
 }
 
 template <int DIM, int NT, int FORMAT>
 static int launch_decode(DecodeParams& p, void* workspace, cudaStream_t st) {
     using S = DecodeShape<DIM, NT>;
-    static_assert(2 * (S::kSmem + 1024 + 256) <= 228 * 1024, "two CTAs per SM");
+    static_assert(S::kCtas * (S::kSmem + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
     CUtensorMap maps[2];
@@ -702,7 +720,7 @@ static int launch_decode(DecodeParams& p, void* workspace, cudaStream_t st) {
         const uint32_t box[3] = {DIM == 64 ? 64u : 128u, (uint32_t)box_rows, 1u};
         if (int rc = make_map(&maps[i], p.c.data[i], 3, dims, strides, box, DIM == 64 ? 64 : 128)) return rc;
     }
-    const int grid = 2 * sms;
+    const int grid = S::kCtas * sms;
     p.meta = static_cast<int32_t*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)grid * 32);
     const int rows = S::kRows;

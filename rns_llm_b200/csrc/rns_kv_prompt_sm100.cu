@@ -990,15 +990,27 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_consta
     const int pieces = meta[1];
     const float* first = p.partial + ((int64_t)blockIdx.x * 2 + meta[2]) * S::kPartial;
     const float* next = p.partial + ((int64_t)blockIdx.x + 1) * 2 * S::kPartial;
-    float top = first[at];
-    for (int i = 1; i < pieces; ++i) top = fmaxf(top, next[(int64_t)(i - 1) * 2 * S::kPartial + at]);
-    float sum = 0.0f, o[DIM / 32] = {};
-    for (int i = 0; i < pieces; ++i) {
-        const float* part = i == 0 ? first : next + (int64_t)(i - 1) * 2 * S::kPartial;
-        const float f = prompt_exp2(part[at] - top);
-        sum = fmaf(part[2 * kTileRows + at], f, sum);
+    const auto piece = [&](int i) { return i == 0 ? first : next + (int64_t)(i - 1) * 2 * S::kPartial; };
+    float top = kNoScore;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, piece(i)[at]);
 #pragma unroll
-        for (int j = 0; j < DIM / 32; ++j) o[j] = fmaf(part[4 * kTileRows + at * DIM + j * 32 + lane], f, o[j]);
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float sum = 0.0f, o[DIM / 32] = {};
+    for (int base = 0; base < pieces; base += 32) {                // pieces in key order, their loads in flight together
+        float mine = 0.0f, total = 0.0f;
+        if (base + lane < pieces) {
+            mine = prompt_exp2(piece(base + lane)[at] - top);
+            total = piece(base + lane)[2 * kTileRows + at];
+        }
+        const int n = min(32, pieces - base);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float* part = piece(base + i) + 4 * kTileRows + at * DIM + lane;
+            const float f = __shfl_sync(0xffffffffu, mine, i);
+            sum = fmaf(__shfl_sync(0xffffffffu, total, i), f, sum);
+#pragma unroll
+            for (int j = 0; j < DIM / 32; ++j) o[j] = fmaf(part[j * 32], f, o[j]);
+        }
     }
     const bool empty = top == kNoScore && sum == 0.0f;
     const float inv = empty ? 0.0f : 1.0f / sum;
