@@ -104,10 +104,21 @@ template <typename T> __device__ __forceinline__ float kv_to_float(T v);
 template <> __device__ __forceinline__ float kv_to_float<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float kv_to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float kv_to_float<float>(float v) { return v; }
-template <typename T> __device__ __forceinline__ T kv_from_float(float v);
-template <> __device__ __forceinline__ __half kv_from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 kv_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ float kv_from_float<float>(float v) { return v; }
+// Two neighbouring elements of a 16-bit type in one word <-> floats.
+template <typename T> __device__ __forceinline__ float2 kv_unpack(uint32_t w);
+template <> __device__ __forceinline__ float2 kv_unpack<__half>(uint32_t w) {
+    return make_float2(__half2float(__ushort_as_half((unsigned short)w)), __half2float(__ushort_as_half((unsigned short)(w >> 16))));
+}
+template <> __device__ __forceinline__ float2 kv_unpack<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint32_t kv_pack(float x, float y);
+template <> __device__ __forceinline__ uint32_t kv_pack<__half>(float x, float y) {
+    return (uint32_t)__half_as_ushort(__float2half_rn(x)) | (uint32_t)__half_as_ushort(__float2half_rn(y)) << 16;
+}
+template <> __device__ __forceinline__ uint32_t kv_pack<__nv_bfloat16>(float x, float y) {
+    return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(x)) | (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(y)) << 16;
+}
 
 // One cached byte <-> float.  Rounding to the grid is to nearest, ties to even, clamped.
 template <int FORMAT> __device__ __forceinline__ float kv_decode(int8_t byte) {
@@ -119,6 +130,66 @@ template <int FORMAT> __device__ __forceinline__ float kv_decode(int8_t byte) {
 template <int FORMAT> __device__ __forceinline__ uint8_t kv_encode(float x) {
     if (FORMAT == RNS_KV_INT8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(x)));
     return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+// Four cached bytes -> floats, exactly.  An integer byte becomes the low mantissa byte of 2^23 + 128 + value: the
+// conversion unit has a quarter of the rate of these.
+template <int FORMAT> __device__ __forceinline__ void kv_decode4(uint32_t w, float (&v)[4]) {
+    if (FORMAT == RNS_KV_INT8) {
+        const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540u + i)), -8388736.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(h));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    }
+}
+// x / scale on the grid, eight values -> bytes; inverse = 1 / scale.  The quotient is the correctly rounded
+// one: the product with the inverse is off by at most two units in the last place, so only values that
+// close to the middle between two grid points need the division.
+template <int FORMAT> __device__ __forceinline__ uint2 kv_encode8(const float (&x)[8], float scale, float inverse) {
+    uint32_t out[2];
+    bool close = false;
+    if (FORMAT == RNS_KV_INT8) {
+        float far = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            uint32_t bits[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float y = __fmul_rn(x[4 * w + i], inverse), t = __fadd_rn(y, kMagic);   // |y| < 128: t's low byte is rint(y)
+                far = fmaxf(far, fabsf(__fsub_rn(y, __fsub_rn(t, kMagic))));
+                bits[i] = __float_as_uint(t);
+            }
+            out[w] = __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+        }
+        close = far > 0.4999f;
+    } else {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            uint32_t lo = 0, hi = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float a = __fmul_rn(x[4 * w + 2 * i], inverse), b = __fmul_rn(x[4 * w + 2 * i + 1], inverse);
+                lo |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a * (1.0f - 0x1p-21f), b * (1.0f - 0x1p-21f)), __NV_SATFINITE, __NV_E4M3) << (16 * i);
+                hi |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a * (1.0f + 0x1p-21f), b * (1.0f + 0x1p-21f)), __NV_SATFINITE, __NV_E4M3) << (16 * i);
+            }
+            close = close || lo != hi;
+            out[w] = lo;
+        }
+    }
+    if (close) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            out[w] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[w] |= (uint32_t)kv_encode<FORMAT>(__fdiv_rn(x[4 * w + i], scale)) << (8 * i);
+        }
+    }
+    return make_uint2(out[0], out[1]);
 }
 #endif
 

@@ -281,7 +281,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int page = half_key < ahead.length ? kv_page(p.c, ahead.b, half_key >> p.c.page_shift) : -1;
                 const uint32_t at = smem_addr(my_scales + ahead_slot * 4 + lane);
                 if (page >= 0) {
-                    const float* src = p.c.scale[side] + (int64_t)page * p.c.kv_heads + ahead.kv_head;
+                    const float* src = (side ? p.c.scale[1] : p.c.scale[0]) + (int64_t)page * p.c.kv_heads + ahead.kv_head;
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(src) : "memory");
                 } else {
                     asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(0.0f) : "memory");

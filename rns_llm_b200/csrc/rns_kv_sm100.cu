@@ -55,25 +55,41 @@ struct KvSource {
 };
 
 // 8 consecutive elements as floats; VECTOR: 16-byte loads (addresses are 16-byte aligned).
-template <typename T, bool VECTOR> __device__ __forceinline__ void kv_load8(const T* p, float (&v)[8]) {
-    if (!VECTOR) {
+template <typename T, bool VECTOR> struct Load8 {
+    static __device__ __forceinline__ void at(const T* p, float (&v)[8]) {
+        if (VECTOR) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            const float2 x = kv_unpack<T>(a.x), y = kv_unpack<T>(a.y), z = kv_unpack<T>(a.z), w = kv_unpack<T>(a.w);
+            v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y; v[4] = z.x; v[5] = z.y; v[6] = w.x; v[7] = w.y;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = kv_to_float<T>(p[i]);
-    } else if (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            T lo, hi;
-            const uint16_t l = (uint16_t)(w[i] & 0xffff), h = (uint16_t)(w[i] >> 16);
-            memcpy(&lo, &l, 2); memcpy(&hi, &h, 2);
-            v[2 * i] = kv_to_float<T>(lo);
-            v[2 * i + 1] = kv_to_float<T>(hi);
+            for (int i = 0; i < 8; ++i) v[i] = kv_to_float<T>(p[i]);
         }
     }
+};
+template <bool VECTOR> struct Load8<float, VECTOR> {
+    static __device__ __forceinline__ void at(const float* p, float (&v)[8]) {
+        if (VECTOR) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p[i];
+        }
+    }
+};
+// 16 floats to 16 consecutive elements at a 16-byte boundary.
+template <typename T> __device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
+    uint4* o = reinterpret_cast<uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        o[i] = make_uint4(kv_pack<T>(v[8 * i], v[8 * i + 1]), kv_pack<T>(v[8 * i + 2], v[8 * i + 3]),
+                          kv_pack<T>(v[8 * i + 4], v[8 * i + 5]), kv_pack<T>(v[8 * i + 6], v[8 * i + 7]));
+}
+template <> __device__ __forceinline__ void store16<float>(float* p, const float (&v)[16]) {
+    float4* o = reinterpret_cast<float4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
 
 constexpr int kWriteVectors = 8;                  // groups of 8 elements a thread holds
@@ -89,16 +105,14 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource sr
     const int nth = (from >> c.page_shift) + blockIdx.x;
     const int page_from = nth << c.page_shift;
     if (page_from >= s.length) return;
-    const int page = kv_page(c, b, nth);
-    if (page < 0) return;
+    const int32_t named = kv_entry(c, b, nth);                     // looked at when the new tokens are on their way
     const int row0 = max(from - page_from, 0), row1 = min(s.length - page_from, c.page_tokens);
-    const int64_t block = (int64_t)page * c.kv_heads + head;
-    int8_t* data = c.data[which] + block * c.page_tokens * c.head_dim;
-    float* scale = c.scale[which] + block;
     const int groups = c.head_dim >> 3;                            // groups of 8 elements in a row
+    // (selects, not indices: an indexed parameter is copied to local memory first)
+    const int64_t token_stride = which ? src.token_stride[1] : src.token_stride[0];
     // element 0 of the block's row 0 (which may lie before the first new token: never read there)
-    const T* x = static_cast<const T*>(src.x[which]) + head * src.head_stride[which] +
-                 (s.begin + page_from - (s.length - s.count)) * src.token_stride[which];
+    const T* x = static_cast<const T*>(which ? src.x[1] : src.x[0]) + head * (which ? src.head_stride[1] : src.head_stride[0]) +
+                 (s.begin + page_from - (s.length - s.count)) * token_stride;
 
     float v[kWriteVectors][8];
     uint32_t top = 0;
@@ -108,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource sr
         const int g = first + t + i * THREADS;
         if (g < last) {
             const int row = g / groups;
-            kv_load8<T, VECTOR>(x + row * src.token_stride[which] + (g - row * groups) * 8, v[i]);
+            Load8<T, VECTOR>::at(x + row * token_stride + (g - row * groups) * 8, v[i]);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
@@ -119,6 +133,11 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource sr
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(fabsf(v[i][e])));
     top = __reduce_max_sync(0xffffffffu, top);
+    const int page = kv_named(c, named);
+    if (page < 0) return;                                          // the whole CTA's page
+    const int64_t block = (int64_t)page * c.kv_heads + head;
+    int8_t* data = (which ? c.data[1] : c.data[0]) + block * c.page_tokens * c.head_dim;
+    float* scale = (which ? c.scale[1] : c.scale[0]) + block;
     __shared__ uint32_t warp_top[THREADS / 32];
     if ((t & 31) == 0) warp_top[t >> 5] = top;
     const float old_scale = row0 > 0 ? *scale : 0.0f;
@@ -143,18 +162,11 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource sr
             words[g] = r;
         }
     }
+    const float inverse = __fdiv_rn(1.0f, s_new);
 #pragma unroll
     for (int i = 0; i < kWriteVectors; ++i) {
         const int g = first + t + i * THREADS;
-        if (g < last) {
-            uint32_t lo = 0, hi = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                lo |= (uint32_t)kv_encode<FORMAT>(__fdiv_rn(v[i][e], s_new)) << (8 * e);
-                hi |= (uint32_t)kv_encode<FORMAT>(__fdiv_rn(v[i][e + 4], s_new)) << (8 * e);
-            }
-            *reinterpret_cast<uint2*>(data + (int64_t)g * 8) = make_uint2(lo, hi);
-        }
+        if (g < last) *reinterpret_cast<uint2*>(data + (int64_t)g * 8) = kv_encode8<FORMAT>(v[i], s_new, inverse);
     }
 }
 
@@ -193,28 +205,44 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(KvView c, const i
     if (at >= count) return;
     const int chunks = c.head_dim >> 4, total = min(chunk_rows, count - at) * chunks;
     T* out = (which ? out_v : out_k) + ((begin + at) * c.kv_heads + head) * c.head_dim;
+    // pages first, then bytes and scales, then the arithmetic: what is independent is in flight together
+    int32_t named[kReadVectors];
+    uint4 q[kReadVectors];
+    float s[kReadVectors];
+#pragma unroll
+    for (int i = 0; i < kReadVectors; ++i) {
+        const int g = threadIdx.x + i * kReadThreads;
+        named[i] = g < total ? kv_entry(c, b, (position + at + g / chunks) >> c.page_shift) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kReadVectors; ++i) {
+        const int g = threadIdx.x + i * kReadThreads;
+        q[i] = make_uint4(0, 0, 0, 0);
+        s[i] = 0.0f;
+        if (g >= total) continue;
+        const int page = kv_named(c, named[i]);
+        if (page >= 0) {
+            const int row = g / chunks, token = position + at + row;
+            const int64_t block = (int64_t)page * c.kv_heads + head;
+            q[i] = *reinterpret_cast<const uint4*>(
+                (which ? c.data[1] : c.data[0]) + (block * c.page_tokens + (token & (c.page_tokens - 1))) * c.head_dim + (g - row * chunks) * 16);
+            s[i] = (which ? c.scale[1] : c.scale[0])[block];
+        }
+    }
 #pragma unroll
     for (int i = 0; i < kReadVectors; ++i) {
         const int g = threadIdx.x + i * kReadThreads;
         if (g >= total) continue;
-        const int row = g / chunks, col = g - row * chunks, token = position + at + row;
-        const int page = kv_page(c, b, token >> c.page_shift);
-        uint4 q = make_uint4(0, 0, 0, 0);
-        float s = 0.0f;
-        if (page >= 0) {
-            const int64_t block = (int64_t)page * c.kv_heads + head;
-            q = *reinterpret_cast<const uint4*>(
-                c.data[which] + (block * c.page_tokens + (token & (c.page_tokens - 1))) * c.head_dim + col * 16);
-            s = c.scale[which][block];
+        const int row = g / chunks, col = g - row * chunks;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float f[4];
+            kv_decode4<FORMAT>(e == 0 ? q[i].x : e == 1 ? q[i].y : e == 2 ? q[i].z : q[i].w, f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[4 * e + k] = __fmul_rn(f[k], s[i]);
         }
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        alignas(16) T v[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-            v[e] = kv_from_float<T>(__fmul_rn(kv_decode<FORMAT>((int8_t)(w[e >> 2] >> (8 * (e & 3)))), s));
-        uint4* o = reinterpret_cast<uint4*>(out + (int64_t)row * c.kv_heads * c.head_dim + col * 16);
-#pragma unroll
-        for (int e = 0; e < (int)sizeof(T); ++e) o[e] = reinterpret_cast<const uint4*>(v)[e];
+        store16<T>(out + (int64_t)row * c.kv_heads * c.head_dim + col * 16, v);
     }
 }
 
