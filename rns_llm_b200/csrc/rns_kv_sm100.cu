@@ -54,28 +54,61 @@ struct KvSource {
     int64_t token_stride[2], head_stride[2];      // elements
 };
 
-// 8 consecutive elements as floats; VECTOR: 16-byte loads (addresses are 16-byte aligned).
-template <typename T, bool VECTOR> struct Load8 {
-    static __device__ __forceinline__ void at(const T* p, float (&v)[8]) {
+// 8 consecutive elements as they lie in memory; VECTOR: 16-byte loads (addresses are 16-byte aligned).  A
+// thread holds its share of a block in this form, half the registers of floats.  `most` gathers the largest
+// magnitude as bits of the type (they order like the numbers, with infinities and NaN on top).
+template <typename T> struct Raw8 {
+    uint32_t w[4];
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
+    template <bool VECTOR> __device__ __forceinline__ void load(const T* p) {
         if (VECTOR) {
             const uint4 a = *reinterpret_cast<const uint4*>(p);
-            const float2 x = kv_unpack<T>(a.x), y = kv_unpack<T>(a.y), z = kv_unpack<T>(a.z), w = kv_unpack<T>(a.w);
-            v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y; v[4] = z.x; v[5] = z.y; v[6] = w.x; v[7] = w.y;
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
         } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = kv_to_float<T>(p[i]);
+            for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ void most(uint32_t& m) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    }
+    // the gathered magnitudes -> bits of the largest as a float
+    static __device__ __forceinline__ uint32_t float_bits(uint32_t m) {
+        return __float_as_uint(kv_unpack<T>(max(m & 0xffffu, m >> 16)).x);
+    }
+    __device__ __forceinline__ void expand(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = kv_unpack<T>(w[i]);
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
         }
     }
 };
-template <bool VECTOR> struct Load8<float, VECTOR> {
-    static __device__ __forceinline__ void at(const float* p, float (&v)[8]) {
+template <> struct Raw8<float> {
+    float w[8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0.0f;
+    }
+    template <bool VECTOR> __device__ __forceinline__ void load(const float* p) {
         if (VECTOR) {
             const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = p[i];
+            for (int i = 0; i < 8; ++i) w[i] = p[i];
         }
+    }
+    __device__ __forceinline__ void most(uint32_t& m) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(w[i]) & 0x7fffffffu);
+    }
+    static __device__ __forceinline__ uint32_t float_bits(uint32_t m) { return m; }
+    __device__ __forceinline__ void expand(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = w[i];
     }
 };
 // 16 floats to 16 consecutive elements at a 16-byte boundary.
@@ -114,25 +147,21 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource sr
     const T* x = static_cast<const T*>(which ? src.x[1] : src.x[0]) + head * (which ? src.head_stride[1] : src.head_stride[0]) +
                  (s.begin + page_from - (s.length - s.count)) * token_stride;
 
-    float v[kWriteVectors][8];
-    uint32_t top = 0;
+    Raw8<T> v[kWriteVectors];
+    uint32_t most = 0;
     const int first = row0 * groups, last = row1 * groups;
 #pragma unroll
     for (int i = 0; i < kWriteVectors; ++i) {
         const int g = first + t + i * THREADS;
+        v[i].clear();
         if (g < last) {
             const int row = g / groups;
-            Load8<T, VECTOR>::at(x + row * token_stride + (g - row * groups) * 8, v[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+            v[i].template load<VECTOR>(x + row * token_stride + (g - row * groups) * 8);
         }
     }
 #pragma unroll
-    for (int i = 0; i < kWriteVectors; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(fabsf(v[i][e])));
-    top = __reduce_max_sync(0xffffffffu, top);
+    for (int i = 0; i < kWriteVectors; ++i) v[i].most(most);
+    uint32_t top = __reduce_max_sync(0xffffffffu, Raw8<T>::float_bits(most));
     const int page = kv_named(c, named);
     if (page < 0) return;                                          // the whole CTA's page
     const int64_t block = (int64_t)page * c.kv_heads + head;
@@ -166,7 +195,11 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource sr
 #pragma unroll
     for (int i = 0; i < kWriteVectors; ++i) {
         const int g = first + t + i * THREADS;
-        if (g < last) *reinterpret_cast<uint2*>(data + (int64_t)g * 8) = kv_encode8<FORMAT>(v[i], s_new, inverse);
+        if (g < last) {
+            float f[8];
+            v[i].expand(f);
+            *reinterpret_cast<uint2*>(data + (int64_t)g * 8) = kv_encode8<FORMAT>(f, s_new, inverse);
+        }
     }
 }
 
