@@ -38,7 +38,13 @@ class QuantizedKVCache:
     v: torch.Tensor
     k_scale: torch.Tensor
     v_scale: torch.Tensor
+    # the struct that calls copy and the shape as plain attributes
     _args: N.KVCacheArgs = field(init=False, repr=False, compare=False)
+    device: torch.device = field(init=False, repr=False, compare=False)
+    pages: int = field(init=False, repr=False, compare=False)
+    kv_heads: int = field(init=False, repr=False, compare=False)
+    page_tokens: int = field(init=False, repr=False, compare=False)
+    head_dim: int = field(init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
         k, v = self.k, self.v
@@ -61,26 +67,7 @@ class QuantizedKVCache:
         self._args = N.KVCacheArgs(d_k=k.data_ptr(), d_v=v.data_ptr(), d_k_scale=self.k_scale.data_ptr(),
                                    d_v_scale=self.v_scale.data_ptr(), pages=pages, page_tokens=page_tokens,
                                    kv_heads=heads, head_dim=dim, format=_FORMATS[k.dtype])
-
-    @property
-    def pages(self) -> int:
-        return self._args.pages
-
-    @property
-    def page_tokens(self) -> int:
-        return self._args.page_tokens
-
-    @property
-    def kv_heads(self) -> int:
-        return self._args.kv_heads
-
-    @property
-    def head_dim(self) -> int:
-        return self._args.head_dim
-
-    @property
-    def device(self) -> torch.device:
-        return self.k.device
+        self.device, self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.device, pages, heads, page_tokens, dim
 
 
 class KVCacheOperators:
@@ -112,7 +99,7 @@ class KVCacheOperators:
             raise ValueError("k and v must be float16, bfloat16 or float32")
         if k.stride(2) != 1 or v.stride(2) != 1:
             raise ValueError("k and v must have unit inner stride")
-        device = cache.k.device
+        device = cache.device
         if k.device != device or v.device != device:
             raise ValueError("k and v must be on the cache's device")
         tokens = k.shape[0]
@@ -122,7 +109,7 @@ class KVCacheOperators:
             N.check(self._lib.rns_kv_write(
                 C.byref(args), k.data_ptr(), v.data_ptr(), _FLOAT_TYPES[k.dtype], tokens, k.stride(0), k.stride(1),
                 v.stride(0), v.stride(1), seq_lens.data_ptr(), query_starts.data_ptr(),
-                _bound(max_query_len, tokens), self._stream(device)))
+                _bound(max_query_len, tokens), _stream(device)))
 
     def kv_cache_read(self, cache: QuantizedKVCache, page_table: torch.Tensor, first: torch.Tensor,
                       row_starts: torch.Tensor, *, rows: int, max_rows: int | None = None,
@@ -137,7 +124,7 @@ class KVCacheOperators:
         if rows < 0:
             raise ValueError("rows must not be negative")
         shape = (rows, cache.kv_heads, cache.head_dim)
-        device = cache.k.device
+        device = cache.device
         if out is None:
             if dtype not in _FLOAT_TYPES:
                 raise ValueError("dtype must be float16, bfloat16 or float32")
@@ -152,7 +139,7 @@ class KVCacheOperators:
         with _on(device):
             N.check(self._lib.rns_kv_read(
                 C.byref(args), first.data_ptr(), row_starts.data_ptr(), rows, _bound(max_rows, rows),
-                out[0].data_ptr(), out[1].data_ptr(), _FLOAT_TYPES[dtype], self._stream(device)))
+                out[0].data_ptr(), out[1].data_ptr(), _FLOAT_TYPES[dtype], _stream(device)))
         return out
 
     def kv_cache_attention(self, q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.Tensor,
@@ -175,7 +162,7 @@ class KVCacheOperators:
             raise ValueError("q must be float16 or bfloat16")
         if q.stride(2) != 1:
             raise ValueError("q must have unit inner stride")
-        device = cache.k.device
+        device = cache.device
         if q.device != device:
             raise ValueError("q must be on the cache's device")
         if window is not None and (window < 1 or not causal):
@@ -205,11 +192,11 @@ class KVCacheOperators:
                 # a captured graph keeps scratch of its own: graphs captured on one stream may be
                 # replayed on two
                 workspace = torch.empty(need, dtype=torch.uint8, device=device)
-                args.d_workspace, stream = workspace.data_ptr(), self._stream(device)
+                args.d_workspace, stream = workspace.data_ptr(), _stream(device)
             elif need:
                 args.d_workspace, stream = self.arena.block(device, need)
             else:
-                stream = self._stream(device)
+                stream = _stream(device)
             args.workspace_bytes = need
             N.check(self._lib.rns_kv_attention(C.byref(cache_args), C.byref(args), stream))
         return (out, lse) if return_lse else out
@@ -217,14 +204,15 @@ class KVCacheOperators:
     def _kv_args(self, cache: QuantizedKVCache, page_table: torch.Tensor, per_sequence: torch.Tensor,
                  starts: torch.Tensor) -> N.KVCacheArgs:
         """The cache with one call's page table, after checking the index tensors."""
-        device = cache.k.device
-        if page_table.ndim != 2 or page_table.dtype != torch.int32 or page_table.device != device or (
-                page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        device = cache.device
+        shape = page_table.shape
+        if len(shape) != 2 or page_table.dtype != torch.int32 or page_table.device != device or (
+                shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be int32 [sequences, pages] on the cache's device, unit inner stride")
-        sequences, width = page_table.shape
+        sequences, width = shape
         for tensor, count in ((per_sequence, sequences), (starts, sequences + 1)):
-            if (tensor.ndim != 1 or tensor.shape[0] != count or tensor.dtype != torch.int32 or
-                    tensor.device != device or not tensor.is_contiguous()):
+            if (tensor.shape != (count,) or tensor.dtype != torch.int32 or tensor.device != device or
+                    not tensor.is_contiguous()):
                 raise ValueError("lengths must be contiguous int32 [sequences] and starts [sequences + 1] on the "
                                  "cache's device")
         args = N.KVCacheArgs.from_buffer_copy(cache._args)
@@ -234,6 +222,10 @@ class KVCacheOperators:
         args.sequences = sequences
         args.d_status = self._state(device).status.data_ptr()
         return args
+
+
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class _Nothing:
@@ -249,7 +241,7 @@ _NOTHING = _Nothing()
 
 def _on(device: torch.device):
     """Makes ``device`` current, when it is not."""
-    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _NOTHING if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _bound(value: int | None, most: int) -> int:

@@ -9,6 +9,8 @@
 
 #include "rns_common.cuh"
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -42,8 +44,10 @@ struct KvQuery {
     float* lse;
 };
 
-// Streaming multiprocessors of the current device.
+// Streaming multiprocessors of the current device; the dynamic shared memory of a kernel, asked for once per
+// device (bits of *done).
 int sm_count(int* out);
+int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done);
 
 // rns_kv_prompt_sm100.cu: sequences with at least min_rows_tokens new tokens, heads of up to 128.
 bool kv_prompt_supported(const KvView& c);

@@ -683,9 +683,23 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ De
 // Host side
 // ---------------------------------------------------------------------------
 int sm_count(int* out) {
+    static std::atomic<int> known[64];                             // per device, looked up once
     int dev = 0;
     RNS_CUDA_OK(cudaGetDevice(&dev));
-    RNS_CUDA_OK(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+    int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        RNS_CUDA_OK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    }
+    *out = n;
+    return RNS_OK;
+}
+int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+    int dev = 0;
+    RNS_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 64 && (done->load(std::memory_order_relaxed) >> dev & 1)) return RNS_OK;
+    RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) done->fetch_or(1ull << dev, std::memory_order_relaxed);
     return RNS_OK;
 }
 
@@ -728,7 +742,8 @@ static int launch_decode(DecodeParams& p, void* workspace, cudaStream_t st) {
     p.token_tile = rows / p.head_tile;
     p.head_tiles = (p.a.group + p.head_tile - 1) / p.head_tile;
     const auto kernel = kv_decode_kernel<DIM, NT, FORMAT>;
-    RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), S::kSmem, &allowed)) return rc;
     kernel<<<grid, kDecodeThreads, S::kSmem, st>>>(maps[0], maps[1], p, box_rows);
     RNS_CUDA_OK(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};

@@ -1057,7 +1057,8 @@ template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* w
     // the kernel's own split of the registers counts on this launch (looked up once per process)
     static const int regs = [&] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0; }();
     if (regs < kLaunchRegs) return fail(RNS_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, not %d", regs, kLaunchRegs);
-    RNS_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), S::kSmem, &allowed)) return rc;
     kernel<<<sms, kPromptThreads, S::kSmem, st>>>(maps[0], maps[1], p);
     RNS_CUDA_OK(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
