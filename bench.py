@@ -623,9 +623,9 @@ def run_opt_decoder(args) -> None:
     seed 1003); fused q|k|v and out_proj of all 12 attention blocks replaced by RNS linears as
     the reference's scripts/evaluate_ppl.py:53-94 does, softmax and FFN in fp16.  Synthetic
     token ids uniform over the vocabulary, batch 8 x 512 tokens of prefill, then 128 greedy
-    decode steps with the key/value cache.  Three variants on the same weights: fp16, native
+    decode steps with the key/value cache.  Variants on the same weights: fp16, native
     int8 (torch._int_mm on the same int8 tensors and scales in the same four linears per
-    block) and RNS.  Reports tokens/s of each and the logits error of the RNS model against
+    block), RNS, and RNS with the keys and values cached in 8 bits.  Reports tokens/s of each and the logits error of the RNS model against
     both; refuses to report when the RNS path did not run (stats counters, as
     scripts/evaluate_ppl.py:212-217)."""
     import copy
@@ -635,7 +635,9 @@ def run_opt_decoder(args) -> None:
     from transformers import OPTConfig, OPTForCausalLM
 
     from rns_llm_b200.backends import CudaRNSBackend
-    from rns_llm_b200.integration import replace_opt_attention_blocks, replace_selected_linears
+    from rns_llm_b200.integration import (replace_opt_attention_blocks, replace_selected_linears,
+                                          use_quantized_cache)
+    from rns_llm_b200.layers import QuantizedDecoderCache
 
     if not torch.cuda.is_available():
         raise SystemExit("bench.py needs a CUDA device; the RNS path has no CPU implementation")
@@ -691,13 +693,15 @@ def run_opt_decoder(args) -> None:
     torch.manual_seed(2003)
     ids = torch.randint(0, config.vocab_size, (batch, prompt), device="cuda")
 
-    def generate(model):
-        """Prefill + greedy decode with the key/value cache; returns (prefill logits of the
-        last position as fp32, seconds of prefill, seconds of decode)."""
+    def generate(model, cache=None):
+        """Prefill + greedy decode with the key/value cache (the model's own, or an 8-bit one);
+        returns (prefill logits of the last position as fp32, seconds of prefill, seconds of decode)."""
+        if cache is not None:
+            cache.reset()
         with torch.no_grad():
             e0, e1, e2 = (torch.cuda.Event(enable_timing=True) for _ in range(3))
             e0.record()
-            out = model(input_ids=ids, use_cache=True)
+            out = model(input_ids=ids, past_key_values=cache, use_cache=True)
             logits = out.logits[:, -1, :].float()
             e1.record()
             cache = out.past_key_values
@@ -710,11 +714,11 @@ def run_opt_decoder(args) -> None:
             torch.cuda.synchronize()
         return logits, e0.elapsed_time(e1) * 1e-3, e1.elapsed_time(e2) * 1e-3
 
-    def measure(model):
-        generate(model)                       # warm-up: weight preparation, arenas, autotuning
+    def measure(model, cache=None):
+        generate(model, cache)                # warm-up: weight preparation, arenas, autotuning
         best = None
         for _ in range(max(1, min(args.steps, 3))):
-            logits, prefill_s, decode_s = generate(model)
+            logits, prefill_s, decode_s = generate(model, cache)
             if best is None or prefill_s + decode_s < best[1] + best[2]:
                 best = (logits, prefill_s, decode_s)
         logits, prefill_s, decode_s = best
@@ -735,7 +739,12 @@ def run_opt_decoder(args) -> None:
     if stats.get("fused_gemm_calls", 0) <= 0 or any(c.projection.compute_count <= 0 for c in coordinators):
         raise SystemExit("the RNS path did not run (fused_gemm_calls / compute_count are zero): nothing to report")
     backend.check_status()
-    del rns_model
+    # the same model with its keys and values in 8 bits as well
+    use_quantized_cache(rns_model)
+    cache = QuantizedDecoderCache.for_model(rns_model, backend, batch=batch, max_tokens=prompt + new_tokens)
+    kv8_logits, results["rns_int8_cache"] = measure(rns_model, cache)
+    backend.check_status()
+    del rns_model, cache
     ffn_model, replaced_ffn, _ = rns_variant(with_ffn=True)
     ffn_logits, results["rns_attention_and_ffn"] = measure(ffn_model)
     backend.check_status()
@@ -757,6 +766,7 @@ def run_opt_decoder(args) -> None:
         "logits_error_last_prefill_position": {
             "rns_vs_fp16": errors(rns_logits, fp16_logits), "rns_vs_int8": errors(rns_logits, int8_logits),
             "int8_vs_fp16": errors(int8_logits, fp16_logits),
+            "rns_int8_cache_vs_rns": errors(kv8_logits, rns_logits),
             "rns_attention_and_ffn_vs_fp16": errors(ffn_logits, fp16_logits)},
         "rns_stats": {k: v for k, v in stats.items() if k.startswith("fused_gemm")},
     }), flush=True)

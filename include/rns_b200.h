@@ -558,7 +558,7 @@ typedef enum rns_kv_format {
  * A cache of `pages` pages and the sequences that a call works on.  A page holds
  * `page_tokens` tokens of every head; the page of one head is a block with one scale.
  *   d_k, d_v              8-bit [pages, kv_heads, page_tokens, head_dim], 16-byte aligned
- *   d_k_scale, d_v_scale  float [pages, kv_heads]
+ *   d_k_scale, d_v_scale  float [pages, kv_heads], not negative
  *   d_page_table          int32 [sequences, table_pages], row stride table_stride: page of
  *                         tokens [i * page_tokens, (i+1) * page_tokens) of a sequence.  Entries
  *                         beyond a sequence's length are not read.

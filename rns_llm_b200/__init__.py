@@ -11,6 +11,8 @@ from .backends import (
 )
 from .layers import (
     CachedRNSQKV,
+    QuantizedCacheAttention,
+    QuantizedDecoderCache,
     RNSLinear,
     RNSQKVProjection,
     install_opt_qkv_fusion,
@@ -27,5 +29,7 @@ __all__ = [
     "RNSLinear",
     "RNSQKVProjection",
     "CachedRNSQKV",
+    "QuantizedCacheAttention",
+    "QuantizedDecoderCache",
     "install_opt_qkv_fusion",
 ]

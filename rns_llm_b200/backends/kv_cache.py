@@ -30,8 +30,9 @@ class QuantizedKVCache:
 
     ``k`` and ``v`` are contiguous ``[pages, kv_heads, page_tokens, head_dim]`` tensors of
     torch.int8 or torch.float8_e4m3fn; ``k_scale`` and ``v_scale`` float32 ``[pages, kv_heads]``:
-    a byte stands for its value times the scale of its page and head.  ``page_tokens`` is 16, 32,
-    64 or 128, ``head_dim`` a multiple of 16 up to 256.
+    a byte stands for its value times the scale of its page and head, which is not negative.
+    ``page_tokens`` is 16, 32, 64 or 128, ``head_dim`` a multiple of 16 up to 256.  The object keeps
+    the addresses of the four tensors it was made with.
     """
 
     k: torch.Tensor
@@ -179,7 +180,7 @@ class KVCacheOperators:
         cache_args = self._kv_args(cache, page_table, seq_lens, query_starts)
         args = N.KVAttentionArgs(
             q.data_ptr(), _FLOAT_TYPES[q.dtype], heads, tokens, q.stride(0), q.stride(1), seq_lens.data_ptr(),
-            query_starts.data_ptr(), _bound(max_query_len, tokens), causal, window or 0,
+            query_starts.data_ptr(), _bound(max_query_len, tokens), causal, min(window or 0, 2 ** 31 - 1),
             dim ** -0.5 if softmax_scale is None else softmax_scale, out.data_ptr(), out.stride(0), out.stride(1),
             None if lse is None else lse.data_ptr(), None, 0)
         self._stats["kv_attention_calls"] += 1

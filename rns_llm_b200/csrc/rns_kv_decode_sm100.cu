@@ -138,8 +138,8 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 }
 // Two bytes in the low halves of x's 16-bit lanes -> fp16 pair.
 __device__ __forceinline__ uint32_t s8_pair(uint32_t x) {
-    uint32_t r = (x & 0x00ff00ffu) ^ 0x64806480u;                 // 1024 + 128 + value
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+    uint32_t r;                                                   // (x & 0x00ff00ff) ^ 0x64806480 = 1024 + 128 + value
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n\tsub.rn.f16x2 %0, %0, %3;" : "=&r"(r) : "r"(x), "r"(0x00ff00ffu), "r"(0x64806480u));
     return r;
 }
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t x) {       // the low 16 bits
@@ -269,6 +269,13 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     int64_t ahead_left = w1 - w0;
     int ahead_step = (int)first_rest, ahead_slot = 0;
     uint32_t flying = 0;                                           // bit s: slot s was issued and not waited for
+    // The page table's entry for the next copy is read one step before it: lanes 0-3, as below.
+    int32_t named = -1;
+    auto look_up = [&]() {
+        const int half_key = ahead.key0 + ahead_step * STEP + warp * KEYS + (KEYS == 32 ? (lane & 1) * 16 : 0);
+        if (lane < 4 && ahead_left > 0 && half_key < ahead.length) named = kv_entry(p.c, ahead.b, half_key >> p.c.page_shift);
+    };
+    look_up();
     auto issue = [&]() {
         if (ahead_left <= 0) return;
         const int key = ahead.key0 + ahead_step * STEP + warp * KEYS;
@@ -278,7 +285,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (lane < 4) {
                 // lane = side * 2 + 16-key half: the half's page and its scale of that side
                 const int side = lane >> 1, half_key = key + (KEYS == 32 ? (lane & 1) * 16 : 0);
-                const int page = half_key < ahead.length ? kv_page(p.c, ahead.b, half_key >> p.c.page_shift) : -1;
+                const int page = half_key < ahead.length ? kv_named(p.c, named) : -1;
                 const uint32_t at = smem_addr(my_scales + ahead_slot * 4 + lane);
                 if (page >= 0) {
                     const float* src = (side ? p.c.scale[1] : p.c.scale[0]) + (int64_t)page * p.c.kv_heads + ahead.kv_head;
@@ -306,9 +313,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             ahead_step = 0;
             decode_next<STEP, KEYS>(p, ahead);
         }
+        look_up();
     };
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < STAGES; ++s) issue();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel may take its place and wait
 
     // --- items
     DecodeItem it = first_item;
@@ -323,22 +332,28 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const int n_tokens = min(p.token_tile, it.count - tile_t0), n_heads = min(p.head_tile, p.a.group - tile_h0);
         const int head0 = it.kv_head * p.a.group + tile_h0;
         // queries of the tile as fp16, each row times a power of two that brings its largest element to [2^7, 2^8)
-        for (int row = warp; row < ROWS; row += kDecodeWarps) {
-            const int tok = row / p.head_tile, hd = row - tok * p.head_tile;
+        // (all of a warp's rows are fetched before the first is looked at: it is their latency that counts)
+        constexpr int MINE = ROWS / kDecodeWarps, PER = DIM / 32;
+        float v[MINE][PER];
+#pragma unroll
+        for (int n = 0; n < MINE; ++n) {
+            const int row = warp + n * kDecodeWarps, tok = row / p.head_tile, hd = row - tok * p.head_tile;
             const bool there = tok < n_tokens && hd < n_heads;
-            float v[DIM / 32];
+            const int64_t at = (it.begin + tile_t0 + tok) * p.a.q_token_stride + (int64_t)(head0 + hd) * p.a.q_head_stride + lane;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                v[n][i] = 0.0f;
+                if (there && lane + i * 32 < p.c.head_dim)
+                    v[n][i] = p.a.type == RNS_F16 ? __half2float(static_cast<const __half*>(p.a.q)[at + i * 32])
+                                                  : __bfloat162float(static_cast<const __nv_bfloat16*>(p.a.q)[at + i * 32]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < MINE; ++n) {
+            const int row = warp + n * kDecodeWarps;
             float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < DIM / 32; ++i) {
-                const int d = lane + i * 32;
-                v[i] = 0.0f;
-                if (there && d < p.c.head_dim) {
-                    const int64_t at = (it.begin + tile_t0 + tok) * p.a.q_token_stride + (int64_t)(head0 + hd) * p.a.q_head_stride + d;
-                    v[i] = p.a.type == RNS_F16 ? __half2float(static_cast<const __half*>(p.a.q)[at])
-                                               : __bfloat162float(static_cast<const __nv_bfloat16*>(p.a.q)[at]);
-                }
-                top = fmaxf(top, fabsf(v[i]));
-            }
+            for (int i = 0; i < PER; ++i) top = fmaxf(top, fabsf(v[n][i]));
             const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
             const int e = (int)(bits >> 23);                       // biased exponent of the largest element
             const bool plain = bits == 0 || e == 255;
@@ -347,7 +362,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             const float up = __uint_as_float((uint32_t)(shift + 127) << 23);
             const float down = __uint_as_float((uint32_t)(127 - max(-120, min(126, shift))) << 23);
 #pragma unroll
-            for (int i = 0; i < DIM / 32; ++i) q_rows[row * (DIM + 8) + lane + i * 32] = __float2half_rn(v[i] * up);
+            for (int i = 0; i < PER; ++i) q_rows[row * (DIM + 8) + lane + i * 32] = __float2half_rn(v[n][i] * up);
             if (lane == 0) row_scale[row] = p.a.scale_log2 * down;
         }
         __syncthreads();
@@ -381,7 +396,18 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const int all_first = p.a.window > 0 ? position + n_tokens - p.a.window : 0;
         const int tile_first = p.a.window > 0 ? position + 1 - p.a.window : 0;
 
-        float o[MT][NT][4], m[NT][2], l[NT][2], v_unit = 0x1p-123f;
+        // and those that each of this thread's rows sees: [sees0, sees1)
+        int sees0[NT][2], sees1[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int pos = position + (nt * 8 + 2 * c4 + e) / p.head_tile;
+                sees1[nt][e] = pos < 0 ? 0 : p.a.causal ? pos + 1 : it.length;
+                sees0[nt][e] = p.a.window > 0 ? pos + 1 - p.a.window : 0;
+            }
+
+        float o[MT][NT][4], m[NT][2], l[NT][2], v_unit = 0x1p-123f, per_unit = 0x1p123f;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -406,11 +432,12 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         const float k_scale = my_scales[slot * 4 + half];
                         float v_scale = my_scales[slot * 4 + 2 + half];
                         if (!(fabsf(v_scale) <= 3.0e38f)) v_scale = __uint_as_float(0x7fc00000u);
-                        float s[NT][4];
+                        // two chains of products for each tile, so that they do not wait for one another
+                        float s[NT][4], s2[NT][4];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+                            for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
 #pragma unroll
                         for (int chunk = 0; chunk < DIM / 64; ++chunk) {
                             // rows r and r + 8; a thread's chunks are 16 bytes, swizzled by the copy
@@ -428,7 +455,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                 if (!QREG) load_q(chunk * 4 + w, f);
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
-                                    mma_f16(s[nt], a0, a1, a2, a3, QREG ? qf[QREG ? chunk * 4 + w : 0][nt][0] : f[nt][0],
+                                    mma_f16(NT < 4 && (w & 1) ? s2[nt] : s[nt], a0, a1, a2, a3, QREG ? qf[QREG ? chunk * 4 + w : 0][nt][0] : f[nt][0],
                                             QREG ? qf[QREG ? chunk * 4 + w : 0][nt][1] : f[nt][1]);
                             }
                         }
@@ -437,24 +464,28 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                s[nt][e] *= q_scale[nt][e & 1] * k_scale;
-                                if (!whole) {
-                                    const int j = k0 + r + (e >> 1) * 8, tok = (nt * 8 + 2 * c4 + (e & 1)) / p.head_tile;
-                                    const int pos = position + tok;
-                                    const bool sees = pos >= 0 && j < (p.a.causal ? pos + 1 : it.length) &&
-                                                      (p.a.window == 0 || j > pos - p.a.window);
-                                    if (!sees) s[nt][e] = -INFINITY;
-                                }
-                                grow = grow || s[nt][e] > m[nt][e & 1] + kLag;
-                            }
+                            for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (q_scale[nt][e & 1] * k_scale);
                         }
+                        if (!whole) {
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int j = k0 + r + (e >> 1) * 8;
+                                    if (j < sees0[nt][e & 1] || j >= sees1[nt][e & 1]) s[nt][e] = -INFINITY;
+                                }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) grow = grow || s[nt][e] > m[nt][e & 1] + kLag;
                         if (__any_sync(0xffffffffu, grow)) {
                             float v_ratio = 1.0f;
                             if (fabsf(v_scale) > 16.0f * v_unit) {
                                 const float unit = __uint_as_float(__float_as_uint(v_scale) & 0x7f800000u);
                                 v_ratio = v_unit / unit;
                                 v_unit = unit;
+                                per_unit = 1.0f / unit;                                // a power of two: exact
                             }
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
@@ -471,7 +502,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                     for (int i = 0; i < MT; ++i) { o[i][nt][e] *= keep * v_ratio; o[i][nt][e + 2] *= keep * v_ratio; }
                                 }
                         }
-                        const float weight = v_scale / v_unit;
+                        const float weight = v_scale * per_unit;
                         uint32_t pf[NT][2];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
@@ -747,7 +778,7 @@ static int launch_decode(DecodeParams& p, void* workspace, cudaStream_t st) {
     kernel<<<grid, kDecodeThreads, S::kSmem, st>>>(maps[0], maps[1], p, box_rows);
     RNS_CUDA_OK(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid, (unsigned)rows);
+    cfg.gridDim = dim3((unsigned)grid, (unsigned)(p.token_tile * p.head_tile));
     cfg.blockDim = dim3(128);
     cfg.stream = st;
     cudaLaunchAttribute attr;

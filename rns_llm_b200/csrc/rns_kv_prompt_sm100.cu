@@ -241,8 +241,8 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t addr, uint32_t block, uint3
     return d;
 }
 __device__ __forceinline__ uint32_t half_pair_s8(uint32_t x) {
-    uint32_t r = (x & 0x00ff00ffu) ^ 0x64806480u;                 // 1024 + 128 + value
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+    uint32_t r;                                                   // (x & 0x00ff00ff) ^ 0x64806480 = 1024 + 128 + value
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n\tsub.rn.f16x2 %0, %0, %3;" : "=&r"(r) : "r"(x), "r"(0x00ff00ffu), "r"(0x64806480u));
     return r;
 }
 __device__ __forceinline__ uint32_t half_pair_e4m3(uint32_t x) {
@@ -484,6 +484,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __syncthreads();
     int32_t* meta = p.meta + (int64_t)blockIdx.x * 8;
     if (t == 0) meta[0] = 0;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel may take its place and wait
 
     if (w0 < w1) {
         volatile int* abort = &abort_word;

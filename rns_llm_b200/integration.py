@@ -12,7 +12,7 @@ from typing import Iterable, Sequence
 
 from torch import nn
 
-from .layers import RNSLinear, install_opt_qkv_fusion
+from .layers import QuantizedCacheAttention, RNSLinear, install_opt_qkv_fusion
 
 
 def find_parent(model: nn.Module, dotted_name: str) -> tuple[nn.Module, str]:
@@ -53,6 +53,20 @@ def replace_opt_attention_blocks(model: nn.Module, *, backend, blocks: int | Non
                                                        adaptive_channels=adaptive_channels).eval()
             replaced.append(f"{name}.out_proj")
     return replaced, coordinators
+
+
+def use_quantized_cache(model: nn.Module) -> list[str]:
+    """Wraps every OPT attention module of ``model`` (those with the four projections, replaced by RNS
+    linears or not) so that it attends over a ``QuantizedDecoderCache`` passed as ``past_key_values``.
+    Returns their names.  No counterpart in the reference, whose cache stays in floating point."""
+    names = [name for name, module in model.named_modules()
+             if all(isinstance(getattr(module, attr, None), nn.Module) for attr in ("q_proj", "k_proj", "v_proj", "out_proj"))]
+    if not names:
+        raise ValueError("the model has no attention modules with q_proj, k_proj, v_proj and out_proj")
+    for name in names:
+        parent, attribute = find_parent(model, name)
+        setattr(parent, attribute, QuantizedCacheAttention(getattr(parent, attribute)).eval())
+    return names
 
 
 def replace_selected_linears(model: nn.Module, *, backend, patterns: Sequence[str], max_layers: int | None = None,

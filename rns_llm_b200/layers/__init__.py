@@ -1,3 +1,4 @@
+from .rns_attention import QuantizedCacheAttention, QuantizedDecoderCache
 from .rns_linear import RNSLinear
 from .rns_qkv import (
     CachedRNSQKV,
@@ -11,5 +12,7 @@ __all__ = [
     "RNSQKVProjection",
     "CachedRNSQKV",
     "InstalledQKVFusion",
+    "QuantizedCacheAttention",
+    "QuantizedDecoderCache",
     "install_opt_qkv_fusion",
 ]

@@ -260,6 +260,8 @@ ATTENTION = [
     ([300], [130], 2, 1, 64, 64, "int8", torch.float16, 0, False),
     ([64, 65, 63], [1, 2, 64], 40, 1, 64, 64, "int8", torch.float16, 1, True),   # forty heads share one, itself only
     ([128, 31], [3, 31], 4, 2, 16, 16, "int8", torch.float16, 0, True),
+    ([70, 3], [3, 1], 130, 1, 64, 64, "int8", torch.float16, 0, True),        # more heads share one than a tile has rows
+    ([129, 257], [128, 129], 2, 2, 128, 32, "e4m3", torch.bfloat16, 2 ** 40, True),   # a window wider than anything
 ]
 
 
@@ -288,6 +290,56 @@ def test_attention(backend, lens, new, heads, kv_heads, dim, page, fmt, dtype, w
                                       max_query_len=max(new), causal=causal, window=window or None)
     assert torch.equal(got3[:starts[-1]], got[:starts[-1]])
     backend.check_status()
+
+
+@pytest.mark.parametrize("new", [2, 75])
+@pytest.mark.parametrize("scale", [-0.25, 0.0, 1e-30, 3.0])
+def test_attention_with_any_scale(backend, new, scale):
+    lens = [140, 75]
+    s = Setup(backend, lens, kv_heads=2, dim=64, page=32, seed=12)
+    q = torch.from_numpy(s.rng.standard_normal((2 * new, 6, 64)).astype(np.float32)).bfloat16()
+    got, lse = backend.kv_cache_attention(q.cuda(), s.cache, s.d_table, s.ints(lens), s.ints(starts_of([new, new])),
+                                          softmax_scale=scale, return_lse=True)
+    check_attention(s, q, [new, new], got, lse, scale=scale, dtype=torch.bfloat16)
+
+
+def test_a_bound_that_is_too_small_costs_time_only(backend):
+    """Attention uses max_query_len to choose its tiles; results do not depend on it."""
+    lens, new = [300, 40], [90, 1]
+    s = Setup(backend, lens, kv_heads=2, dim=64, page=32, seed=13)
+    q = torch.from_numpy(s.rng.standard_normal((91, 4, 64)).astype(np.float32)).half()
+    for bound in (0, 1, 5, 90, 1000):
+        got = backend.kv_cache_attention(q.cuda(), s.cache, s.d_table, s.ints(lens), s.ints(starts_of(new)), max_query_len=bound)
+        check_attention(s, q, new, got, None, scale=0.125, dtype=torch.float16)
+    backend.check_status()
+
+
+def test_many_sequences(backend):
+    """More sequences than threads of a block, most of them empty or without queries."""
+    rng = np.random.default_rng(3)
+    lens = [int(n) if keep else 0 for n, keep in zip(rng.integers(1, 40, 1300), rng.random(1300) < 0.3)]
+    new = [int(rng.integers(0, 3)) for _ in lens]
+    s = Setup(backend, lens, kv_heads=1, dim=16, page=16, seed=14)
+    q = torch.from_numpy(s.rng.standard_normal((sum(new), 2, 16)).astype(np.float32)).half()
+    for bound in (2, 40):                                        # the rows kernel; the prompt kernel (by its bound)
+        got, lse = backend.kv_cache_attention(q.cuda(), s.cache, s.d_table, s.ints(lens), s.ints(starts_of(new)),
+                                              max_query_len=bound, return_lse=True)
+        check_attention(s, q, new, got, lse, scale=0.25, dtype=torch.float16)
+
+
+def test_other_device_and_stream_are_left_alone(backend):
+    """The call runs on the current stream of the cache's device and leaves both as they were."""
+    s = Setup(backend, [100], kv_heads=2, dim=64, page=32, seed=15)
+    q = torch.from_numpy(s.rng.standard_normal((1, 4, 64)).astype(np.float32)).half().cuda()
+    lens, starts = s.ints([100]), s.ints([0, 1])
+    want = backend.kv_cache_attention(q, s.cache, s.d_table, lens, starts)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = backend.kv_cache_attention(q, s.cache, s.d_table, lens, starts)
+        assert torch.cuda.current_stream() == side
+    side.synchronize()
+    assert torch.equal(got, want) and torch.cuda.current_device() == 0
 
 
 @pytest.mark.parametrize("new", [1, 70])
