@@ -146,7 +146,7 @@ template <int DIM> struct PromptShape {
     static constexpr int kParts = DIM / 64;                        // 64-dimension parts of a tile
     static constexpr int kTile = kBlock * DIM * 2;                 // fp16 tile of keys or values
     static constexpr int kRaw = kBlock * DIM;                      // the same in 8 bits
-    static constexpr int kRing = DIM == 64 ? 4 : 3, kRawRing = 4;
+    static constexpr int kRing = 4, kRawRing = DIM == 64 ? 4 : 2;
     static constexpr int kQ = 2 * kTileRows * DIM * 2;
     static constexpr int kSmem = 1024 + kQ + kRing * kTile + kRawRing * kRaw;
     static constexpr int kPartial = 2 * kTileRows * (DIM + 2);
