@@ -65,6 +65,11 @@ class StreamArena:
         stream = int(torch.cuda.current_stream(index).cuda_stream)
         return self._buffer((index, stream), int(nbytes)).data_ptr(), stream
 
+    def buffer(self, index: int, stream: int, nbytes: int) -> torch.Tensor:
+        """At least ``nbytes`` of the scratch of stream handle ``stream`` on device ``index``, for
+        callers that know both already."""
+        return self._buffer((index, stream), nbytes)
+
     def _buffer(self, key: tuple[int, int], need: int) -> torch.Tensor:
         buf = self._buffers.get(key)
         if buf is not None and buf.numel() >= need:

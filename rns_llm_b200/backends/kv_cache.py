@@ -188,17 +188,16 @@ class KVCacheOperators:
             need = self._lib.rns_kv_attention_workspace(C.byref(cache_args), C.byref(args))
             if need < 0:
                 N.check(-need)
-            workspace = None
-            if need and torch.cuda.is_current_stream_capturing():
-                # a captured graph keeps scratch of its own: graphs captured on one stream may be
-                # replayed on two
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-                args.d_workspace, stream = workspace.data_ptr(), _stream(device)
-            elif need:
-                args.d_workspace, stream = self.arena.block(device, need)
-            else:
-                stream = _stream(device)
-            args.workspace_bytes = need
+            stream = _stream(device)
+            if need:
+                if torch.cuda.is_current_stream_capturing():
+                    # a captured graph keeps scratch of its own: graphs captured on one stream may be
+                    # replayed on two
+                    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+                else:
+                    workspace = self.arena.buffer(device.index, stream, need)
+                args.d_workspace = workspace.data_ptr()
+                args.workspace_bytes = need
             N.check(self._lib.rns_kv_attention(C.byref(cache_args), C.byref(args), stream))
         return (out, lse) if return_lse else out
 
