@@ -208,10 +208,15 @@ static int launch_write(const KvView& c, const KvSource& src, const int32_t* len
                         int64_t tokens, int max_new, bool vector, cudaStream_t st) {
     const dim3 grid((unsigned)((max_new + c.page_tokens - 2) / c.page_tokens + 1), (unsigned)(2 * c.kv_heads),
                     (unsigned)c.sequences);
-    const bool large = c.page_tokens * c.head_dim / 8 > 128 * kWriteVectors;
-    if (vector && !large) kv_write_kernel<T, FORMAT, true, 128><<<grid, 128, 0, st>>>(c, src, lens, starts, tokens, max_new);
-    else if (vector) kv_write_kernel<T, FORMAT, true, 512><<<grid, 512, 0, st>>>(c, src, lens, starts, tokens, max_new);
-    else kv_write_kernel<T, FORMAT, false, 512><<<grid, 512, 0, st>>>(c, src, lens, starts, tokens, max_new);
+    // A CTA holds its block in registers, eight groups of eight elements a thread: the fewest threads that can,
+    // so that an SM has many blocks in flight (pages of 32 x 128, bf16 to e4m3: 43 us with 128 threads, 36 with 64).
+    const int groups = c.page_tokens * c.head_dim / 8;
+#define RNS_KV_WRITE_LAUNCH(V, N) kv_write_kernel<T, FORMAT, V, N><<<grid, N, 0, st>>>(c, src, lens, starts, tokens, max_new)
+    if (!vector) RNS_KV_WRITE_LAUNCH(false, 512);
+    else if (groups <= 64 * kWriteVectors) RNS_KV_WRITE_LAUNCH(true, 64);
+    else if (groups <= 128 * kWriteVectors) RNS_KV_WRITE_LAUNCH(true, 128);
+    else RNS_KV_WRITE_LAUNCH(true, 512);
+#undef RNS_KV_WRITE_LAUNCH
     RNS_CUDA_OK(cudaGetLastError());
     return RNS_OK;
 }
