@@ -27,6 +27,10 @@
 //   is lost, and the accumulators are rescaled only when a vote finds a larger score.  The maximum of
 //   a row follows that row's scores alone, and units are powers of two: but for weights below fp16's
 //   normal range, what a row gives does not depend on the rows beside it.
+//
+// Measured (graph replay): 64 sequences of 1..8192 tokens, 32 over 8 heads of 128, 143 us = 3.75 TB/s of cache
+// (0.58 of the copy rate; 450 instructions for 16 keys, issue slots 53 % busy with three warps a scheduler: the
+// latency of dependent instructions bounds it); one sequence of 131072, e4m3, 68 us; 8 of 640, 12 heads of 64, 16 us.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 
@@ -168,7 +172,9 @@ template <int DIM, int NT> struct DecodeShape {
     static constexpr int kKeys = DIM == 256 ? 16 : 32;             // keys of a warp's stage
     static constexpr int kStep = kKeys * kDecodeWarps;
     static constexpr int kHalf = kKeys * DIM;                      // bytes of one side of a stage
-    static constexpr int kCtas = DIM * NT <= 128 ? 3 : 2;          // CTAs of an SM
+    // CTAs of an SM: three where the accumulators leave registers for it (64 sequences up to 8k: 149 us, 173 with
+    // two; four, with half the keys a stage, 177)
+    static constexpr int kCtas = DIM * NT <= 128 ? 3 : 2;
     static constexpr int kStages = kCtas == 3 ? (DIM == 64 ? 4 : 2) : DIM == 64 ? (NT == 4 ? 5 : 6) : (NT >= 3 || DIM * NT > 256) ? 2 : 3;
     static constexpr int kRing = kDecodeWarps * kStages * 2 * kHalf;
     static constexpr int kStride = DIM + 4;                        // floats between rows of the merge buffer
