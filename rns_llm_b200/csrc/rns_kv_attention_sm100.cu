@@ -21,7 +21,7 @@ static int check_attention(const rns_kv_cache* cache, const rns_kv_attention_arg
         return fail(RNS_ERR_INVALID_ARGUMENT, "token counts must be in [0, 2^31)");
     if (a->window < 0 || (a->window > 0 && !a->causal))
         return fail(RNS_ERR_INVALID_ARGUMENT, "window must not be negative and needs causal");
-    if (!(std::fabs(a->softmax_scale) <= 3.0e38f)) return fail(RNS_ERR_INVALID_ARGUMENT, "softmax_scale must be finite");
+    if (!(std::fabs(a->softmax_scale) <= 2.0e38f)) return fail(RNS_ERR_INVALID_ARGUMENT, "softmax_scale must be finite");
     if (a->tokens > 0 && c->sequences > 0 && (!a->d_q || !a->d_out || !a->d_seq_lens || !a->d_query_starts))
         return fail(RNS_ERR_INVALID_ARGUMENT, "a pointer is NULL");
     memset(p, 0, sizeof(*p));
@@ -41,6 +41,7 @@ static int check_attention(const rns_kv_cache* cache, const rns_kv_attention_arg
 struct Routing {
     bool rows, prompt;
     int rows_most;                 // new tokens of a sequence that the rows kernel takes, at most
+    int rows_new;                  // and those its tiles (and so its workspace) are made for
     int64_t rows_bytes, prompt_bytes;
 };
 static int route(const KvView& c, const KvQuery& a, int max_new, Routing* r) {
@@ -57,7 +58,8 @@ static int route(const KvView& c, const KvQuery& a, int max_new, Routing* r) {
     } else {
         r->rows = true;
     }
-    if (r->rows) r->rows_bytes = kv_decode_workspace(c, a, r->prompt ? r->rows_most : max_new);
+    r->rows_new = r->prompt ? r->rows_most : max_new;
+    if (r->rows) r->rows_bytes = kv_decode_workspace(c, a, r->rows_new);
     if (r->prompt) r->prompt_bytes = kv_prompt_workspace(c);
     if (r->rows_bytes < 0 || r->prompt_bytes < 0) return RNS_ERR_CUDA;
     return RNS_OK;
@@ -92,6 +94,6 @@ extern "C" int rns_kv_attention(const rns_kv_cache* cache, const rns_kv_attentio
     if (r.prompt)
         if (int rc = kv_prompt(c, p, cache->format, r.rows ? r.rows_most + 1 : 0, a->d_workspace, st)) return rc;
     if (r.rows)
-        return kv_decode(c, p, cache->format, r.prompt ? r.rows_most : a->max_new, r.rows_most, a->d_workspace, st);
+        return kv_decode(c, p, cache->format, r.rows_new, r.rows_most, a->d_workspace, st);
     return RNS_OK;
 }

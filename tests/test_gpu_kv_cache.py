@@ -314,6 +314,34 @@ def test_a_bound_that_is_too_small_costs_time_only(backend):
     backend.check_status()
 
 
+@pytest.mark.parametrize("new,bound", [(1, 2 ** 30), (2, 2 ** 31 - 1), (70, 2 ** 30)])
+def test_workspace_covers_any_bound(backend, new, bound):
+    """The C entry with a bound beyond the tokens stays inside the bytes that it asked for."""
+    import ctypes as C
+    from rns_llm_b200 import _native as N
+
+    s = Setup(backend, [5000], kv_heads=2, dim=64, page=64, seed=16)
+    q = torch.from_numpy(s.rng.standard_normal((new, 8, 64)).astype(np.float32)).half().cuda()
+    lens, starts, out = s.ints([5000]), s.ints([0, new]), torch.empty_like(q)
+    cache = backend._kv_args(s.cache, s.d_table, lens, starts)
+    args = N.KVAttentionArgs(q.data_ptr(), N.F16, 8, new, q.stride(0), q.stride(1), lens.data_ptr(), starts.data_ptr(), bound,
+                             1, 0, 0.125, out.data_ptr(), out.stride(0), out.stride(1), None, None, 0)
+    lib = N.load()
+    need = lib.rns_kv_attention_workspace(C.byref(cache), C.byref(args))
+    work = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+    args.d_workspace, args.workspace_bytes = work.data_ptr(), need
+    stream = torch.cuda.current_stream().cuda_stream
+    N.check(lib.rns_kv_attention(C.byref(cache), C.byref(args), stream))
+    assert (work[need:] == 0x5a).all()
+    check_attention(s, q.cpu(), [new], out, None, scale=0.125, dtype=torch.float16)
+    for bad in (dict(workspace_bytes=need - 1), dict(d_workspace=work.data_ptr() + 8), dict(d_workspace=None)):
+        for name, value in bad.items():
+            kept = getattr(args, name)
+            setattr(args, name, value)
+            assert lib.rns_kv_attention(C.byref(cache), C.byref(args), stream) == N.ERR_INVALID_ARGUMENT
+            setattr(args, name, kept)
+
+
 def test_many_sequences(backend):
     """More sequences than threads of a block, most of them empty or without queries."""
     rng = np.random.default_rng(3)
