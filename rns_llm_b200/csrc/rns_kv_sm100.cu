@@ -131,8 +131,9 @@ template <> __device__ __forceinline__ void store16<float>(float* p, const float
 
 constexpr int kWriteVectors = 8;                  // groups of 8 elements a thread holds
 
+// (registers for 1024 threads an SM where the block is held in 16-bit words)
 template <typename T, int FORMAT, bool VECTOR, int THREADS>
-__global__ void __launch_bounds__(THREADS) kv_write_kernel(KvView c, KvSource src, const int32_t* lens,
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VECTOR ? 1024 / THREADS : 1) kv_write_kernel(KvView c, KvSource src, const int32_t* lens,
                                                            const int32_t* starts, int64_t tokens, int max_new) {
     const int b = blockIdx.z, head = blockIdx.y >> 1, which = blockIdx.y & 1, t = threadIdx.x;
     const KvSpan s = kv_span(c, lens, starts, tokens, b);
