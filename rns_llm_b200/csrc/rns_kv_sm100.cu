@@ -10,9 +10,9 @@
 // A block has one owner (a CTA), so nothing is exchanged between CTAs and the result does not
 // depend on any order.
 //
-// Both directions are bound by memory: writing 4096 tokens x 32 heads x 128 (fp16 to int8) takes 27 us, 0.57 of
+// Both directions are bound by memory: writing 4096 tokens x 32 heads x 128 (fp16 to int8) takes 26 us, 0.59 of
 // the copy rate (a CTA's load, reduction and store follow one another, so the number of CTAs in flight counts:
-// 55 us with the block held as floats); reading 65537 x 8 x 128 to bf16 80 us, 0.78 of it.
+// 55 us with the block held as floats); reading 65537 x 8 x 128 to bf16 78 us, 0.79 of it.
 #include "rns_kv.cuh"
 
 namespace rns {
@@ -229,7 +229,9 @@ static int launch_write(const KvView& c, const KvSource& src, const int32_t* len
 // ---------------------------------------------------------------------------
 // read
 // ---------------------------------------------------------------------------
-constexpr int kReadThreads = 256, kReadVectors = 4;   // 16 bytes each: 16 KB of the cache per CTA
+// 16 bytes each: 8 KB of the cache per CTA.  8 x 640 tokens of 12 heads / 65537 of 8 take 8.3 / 78 us; with 256
+// threads 10.1 / 80, with 8 groups of those a thread 14.4 / 104, with 2 of 128 8.3 / 82.
+constexpr int kReadThreads = 128, kReadVectors = 4;
 
 template <typename T, int FORMAT>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(KvView c, const int32_t* first, const int32_t* row_starts,
