@@ -49,8 +49,7 @@ struct KvQuery {
 int sm_count(int* out);
 int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done);
 
-// rns_kv_prompt_sm100.cu: sequences with at least min_rows_tokens new tokens, heads of up to 128.
-bool kv_prompt_supported(const KvView& c);
+// rns_kv_prompt_sm100.cu: sequences with at least min_rows_tokens new tokens.
 int64_t kv_prompt_workspace(const KvView& c);
 int kv_prompt(const KvView& c, const KvQuery& a, int format, int min_rows_tokens, void* workspace, cudaStream_t st);
 

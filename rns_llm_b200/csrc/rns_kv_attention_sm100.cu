@@ -36,8 +36,9 @@ static int check_attention(const rns_kv_cache* cache, const rns_kv_attention_arg
 }
 
 // Which kernel serves which sequences: tiles of the rows kernel hold up to 32 query rows (new tokens x
-// heads that share one of the cache), those of the prompt kernel 256.  Beyond 32 rows the rows kernel reads a
-// sequence's keys once for every tile (8 prompts of 512: 182 us there, 38 us in the prompt kernel).
+// heads that share one of the cache), those of the prompt kernel 256 (128 of heads above 128).  Beyond 32 rows
+// the rows kernel reads a sequence's keys once for every tile (8 prompts of 512: 182 us there, 38 us in the
+// prompt kernel; 48 rows of heads of 256, four sequences of 8000 tokens: 83 and 70 us).
 struct Routing {
     bool rows, prompt;
     int rows_most;                 // new tokens of a sequence that the rows kernel takes, at most
@@ -49,7 +50,7 @@ static int route(const KvView& c, const KvQuery& a, int max_new, Routing* r) {
     r->rows_bytes = r->prompt_bytes = 0;
     r->rows_most = INT32_MAX;
     if (max_new > a.tokens) max_new = (int)a.tokens;
-    if (kv_prompt_supported(c) && (int64_t)max_new * a.group > 32) {
+    if ((int64_t)max_new * a.group > 32) {
         r->prompt = true;
         r->rows_most = 32 / a.group;
         // few sequences can be much shorter than the longest: the prompt kernel takes them all

@@ -1,5 +1,4 @@
-// Attention of many query rows per sequence over the paged 8-bit cache (prompts and chunks of them),
-// heads of up to 128.
+// Attention of many query rows per sequence over the paged 8-bit cache (prompts and chunks of them).
 //
 // A CTA works on two tiles of 128 query rows of one head of the cache (tokens x the heads that share
 // it) and walks the keys in blocks of 128.  Per block and tile:
@@ -9,7 +8,8 @@
 // The bound is the tensor pipe (4 * 128 * 128 * head_dim operations a block and tile), with the
 // exponentials (16 a clock and SM) close behind; bytes from memory hardly count, since a block serves
 // 256 rows.  The two tiles keep the pipe busy in turn: one is multiplied while the other is
-// exponentiated.
+// exponentiated.  Heads above 128 have one tile, as O of one is half of the tensor memory and the fp16
+// tiles of a block are 64 KB each; the warps of the second tile then have nothing to do.
 //
 // * The tensor cores have no product of fp16 with 8-bit operands, so four warps turn each 8-bit tile,
 //   as TMA brought it, into an fp16 tile in the swizzled layout of an operand: exactly, in whatever
@@ -26,6 +26,8 @@
 // prompt of 4096 tokens of 32 heads 229 us; 8 prompts of 512 of 12 heads of 64 38 us.  In steady state a block
 // of both tiles takes 4850 cycles, 2048 of them on the tensor pipe: what bounds it is the chain of one tile,
 // scores -> 430 cycles for the largest -> 2250 for the weights -> second product -> next scores.
+// Heads of 256, where nothing overlaps that chain: a prompt of 2048 tokens of 16 heads 130 us (653 in the rows
+// kernel), 509 tokens behind 8192, 16 over 4 heads, 166 us = 416 TFLOP/s (570 in the rows kernel).
 //
 // Warps 0-3 and 4-7: softmax of a tile, a thread a row (the same warps fetch the queries and store the
 // outputs); 8-11: conversion; 12: issues the products; 13: copies; 14: scales of the pages; 15: the list of
@@ -55,6 +57,7 @@ struct PromptParams {
     KvView c;
     KvQuery a;
     int head_tile, token_tile, head_tiles;
+    int tiles;                            // of an item: 2, or 1 where O fills the tensor memory
     int min_rows_tokens;                  // sequences with fewer new tokens are left to the rows kernel
     int box_rows;
     float sign;                           // of the softmax scale, which is folded into the queries
@@ -77,10 +80,10 @@ __device__ __forceinline__ bool prompt_sequence(const PromptParams& p, int b, Pr
     return s.count >= p.min_rows_tokens && s.count > 0;
 }
 __device__ __forceinline__ int prompt_pairs(const PromptParams& p, int count) {
-    return (count + 2 * p.token_tile - 1) / (2 * p.token_tile) * p.head_tiles;
+    return (count + p.tiles * p.token_tile - 1) / (p.tiles * p.token_tile) * p.head_tiles;
 }
 __device__ __forceinline__ void prompt_range(const PromptParams& p, PromptItem& it) {
-    it.token0 = it.pair / p.head_tiles * 2 * p.token_tile;
+    it.token0 = it.pair / p.head_tiles * p.tiles * p.token_tile;
     it.head0 = it.pair % p.head_tiles * p.head_tile;
     const int base = it.length - it.count;
     int first[2], last[2], low = INT32_MAX, high = 0;
@@ -89,7 +92,7 @@ __device__ __forceinline__ void prompt_range(const PromptParams& p, PromptItem& 
         const int ta = it.token0 + i * p.token_tile, tb = min(ta + p.token_tile, it.count);
         first[i] = p.a.window > 0 ? max(0, base + ta - p.a.window + 1) : 0;
         last[i] = p.a.causal ? base + tb : it.length;
-        if (ta >= it.count || base + tb <= 0) last[i] = 0;
+        if (i >= p.tiles || ta >= it.count || base + tb <= 0) last[i] = 0;
         if (last[i] > first[i]) { low = min(low, first[i]); high = max(high, last[i]); }
     }
     it.low = low;
@@ -159,10 +162,11 @@ __device__ __forceinline__ void prompt_next(const PromptParams& p, PromptPart& p
 
 template <int DIM> struct PromptShape {
     static constexpr int kParts = DIM / 64;                        // 64-dimension parts of a tile
+    static constexpr int kTiles = DIM == 256 ? 1 : 2;              // tiles of an item: S of each and O of each in 512 columns
     static constexpr int kTile = kBlock * DIM * 2;                 // fp16 tile of keys or values
     static constexpr int kRaw = kBlock * DIM;                      // the same in 8 bits
-    static constexpr int kRing = 4, kRawRing = DIM == 64 ? 4 : 2;
-    static constexpr int kQ = 2 * kTileRows * DIM * 2;
+    static constexpr int kRing = DIM == 256 ? 2 : 4, kRawRing = DIM == 64 ? 4 : DIM == 128 ? 2 : 1;
+    static constexpr int kQTile = kTileRows * DIM * 2, kQ = kTiles * kQTile;
     static constexpr int kSmem = 1024 + kQ + kRing * kTile + kRawRing * kRaw;
     static constexpr int kPartial = 2 * kTileRows * (DIM + 2);
     static constexpr int kO = 256;                                 // tensor memory: S/P of the tiles at 0 and 128, O from here
@@ -579,7 +583,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         const __half2 f = __floats2half2_rn(v[a] * up, v[b] * up);
                         h[i] = *reinterpret_cast<const uint32_t*>(&f);
                     }
-                    const uint32_t to = q_smem + tile * (S::kQ / 2) + (c >> 3) * (kTileRows * 128) + row * 128 +
+                    const uint32_t to = q_smem + tile * S::kQTile + (c >> 3) * (kTileRows * 128) + row * 128 +
                                         (((c & 7) ^ (row & 7)) << 4);
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                 }
@@ -671,7 +675,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 // the row's output: to its place, or as a piece of it (largest score, sum, O) to the workspace
                 const bool complete = part.step == 0 && part.stop == it.blocks, empty = m == kNoScore && l == 0.0f;
-                const bool there = row_token < p.token_tile && it.token0 + tile * p.token_tile + row_token < it.count &&
+                const bool there = tile < S::kTiles && row_token < p.token_tile && it.token0 + tile * p.token_tile + row_token < it.count &&
                                    it.head0 + row_head < p.a.group;
                 const int64_t token = it.begin + it.token0 + tile * p.token_tile + row_token;
                 const int64_t head = (int64_t)it.kv_head * p.a.group + it.head0 + row_head;
@@ -773,7 +777,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll 2
                         for (int u = warp - kConvertWarp; u < kBlock / 8 * S::kParts; u += 4) {
                             const int part64 = u % S::kParts, keys = u / S::kParts * 8;
-                            const uint32_t at = from + keys * DIM + raw_at + (DIM == 128 ? (part64 << 6 ^ raw_flip) : 0);
+                            const uint32_t at = DIM == 64 ? from + keys * 64 + raw_at
+                                                          : from + (part64 >> 1) * (kBlock * 128) + keys * 128 + raw_at + ((part64 & 1) << 6 ^ raw_flip);
                             uint32_t w[4];
                             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
                             // bytes behind the sequence may be NaN patterns, which no weight of zero removes
@@ -842,7 +847,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                             if (!ok) break;
                         }
                         const uint32_t s_d = tm + tile * 128, o_d = tm + S::kO + tile * DIM;
-                        const uint64_t q_desc = q0 + tile * (S::kQ / 2 >> 4);
+                        const uint64_t q_desc = q0 + tile * (S::kQTile >> 4);
                         if (elect_one()) {
                             if (second) {
 #pragma unroll
@@ -907,9 +912,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         const uint32_t bar = smem_addr(&bars.raw_full[rs]);
                         if (lane == 0) mbar_arrive_expect_tx(bar, S::kRaw);
                         __syncwarp();
-                        if ((lane >> 3) == (u >> 1) && box < boxes)
-                            tma_load_3d(raw + rs * S::kRaw + box * p.box_rows * DIM, side ? &map_v : &map_k, bar, 0,
-                                        kv_head * p.c.page_tokens + (key & (p.c.page_tokens - 1)), z);
+                        if ((lane >> 3) == (u >> 1) && box < boxes) {
+                            const uint32_t to = raw + rs * S::kRaw + box * p.box_rows * (DIM == 64 ? 64 : 128);
+                            const int y = kv_head * p.c.page_tokens + (key & (p.c.page_tokens - 1));
+                            tma_load_3d(to, side ? &map_v : &map_k, bar, 0, y, z);
+                            if (DIM == 256) tma_load_3d(to + kBlock * 128, side ? &map_v : &map_k, bar, 128, y, z);
+                        }
                     }
                 }
                 part_done();
@@ -1005,7 +1013,7 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_consta
     const int row_token = row / p.head_tile, row_head = row - row_token * p.head_tile;
     const KvSpan s = kv_span(p.c, p.a.lens, p.a.starts, p.a.tokens, meta[3]);
     const int tok = meta[5] + tile * p.token_tile + row_token, hd = meta[6] + row_head;
-    if (row_token >= p.token_tile || tok >= s.count || hd >= p.a.group) return;
+    if (tile >= S::kTiles || row_token >= p.token_tile || tok >= s.count || hd >= p.a.group) return;
     const int pieces = meta[1];
     const float* first = p.partial + ((int64_t)blockIdx.x * 2 + meta[2]) * S::kPartial;
     const float* next = p.partial + ((int64_t)blockIdx.x + 1) * 2 * S::kPartial;
@@ -1049,12 +1057,11 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_consta
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-bool kv_prompt_supported(const KvView& c) { return c.head_dim <= 128; }
-
 int64_t kv_prompt_workspace(const KvView& c) {
     int sms = 0;
     if (sm_count(&sms) != RNS_OK) return -RNS_ERR_CUDA;
-    return (int64_t)sms * (2 * (c.head_dim <= 64 ? PromptShape<64>::kPartial : PromptShape<128>::kPartial) * 4 + 32);
+    const int piece = c.head_dim <= 64 ? PromptShape<64>::kPartial : c.head_dim <= 128 ? PromptShape<128>::kPartial : PromptShape<256>::kPartial;
+    return (int64_t)sms * (2 * piece * 4 + 32);
 }
 
 template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* workspace, cudaStream_t st) {
@@ -1063,12 +1070,13 @@ template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* w
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
     p.box_rows = p.c.page_tokens;
+    p.tiles = S::kTiles;
     CUtensorMap maps[2];
     for (int i = 0; i < 2; ++i) {
         const uint64_t dims[3] = {(uint64_t)p.c.head_dim, (uint64_t)p.c.kv_heads * p.c.page_tokens, (uint64_t)p.c.pages};
         const uint64_t strides[2] = {dims[0], dims[0] * dims[1]};
-        const uint32_t box[3] = {(uint32_t)DIM, (uint32_t)p.box_rows, 1u};
-        if (int rc = make_map(&maps[i], p.c.data[i], 3, dims, strides, box, DIM)) return rc;
+        const uint32_t box[3] = {DIM == 64 ? 64u : 128u, (uint32_t)p.box_rows, 1u};
+        if (int rc = make_map(&maps[i], p.c.data[i], 3, dims, strides, box, DIM == 64 ? 64 : 128)) return rc;
     }
     p.meta = static_cast<int32_t*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)sms * 32);
@@ -1104,7 +1112,9 @@ int kv_prompt(const KvView& c, const KvQuery& a, int format, int min_rows_tokens
     p.head_tiles = (a.group + p.head_tile - 1) / p.head_tile;
     if (c.head_dim <= 64)
         return format == RNS_KV_INT8 ? launch_prompt<64, RNS_KV_INT8>(p, workspace, st) : launch_prompt<64, RNS_KV_E4M3>(p, workspace, st);
-    return format == RNS_KV_INT8 ? launch_prompt<128, RNS_KV_INT8>(p, workspace, st) : launch_prompt<128, RNS_KV_E4M3>(p, workspace, st);
+    if (c.head_dim <= 128)
+        return format == RNS_KV_INT8 ? launch_prompt<128, RNS_KV_INT8>(p, workspace, st) : launch_prompt<128, RNS_KV_E4M3>(p, workspace, st);
+    return format == RNS_KV_INT8 ? launch_prompt<256, RNS_KV_INT8>(p, workspace, st) : launch_prompt<256, RNS_KV_E4M3>(p, workspace, st);
 }
 
 }  // namespace rns

@@ -262,6 +262,11 @@ ATTENTION = [
     ([128, 31], [3, 31], 4, 2, 16, 16, "int8", torch.float16, 0, True),
     ([70, 3], [3, 1], 130, 1, 64, 64, "int8", torch.float16, 0, True),        # more heads share one than a tile has rows
     ([129, 257], [128, 129], 2, 2, 128, 32, "e4m3", torch.bfloat16, 2 ** 40, True),   # a window wider than anything
+    ([700, 300, 0, 129], [300, 299, 0, 1], 6, 2, 256, 64, "e4m3", torch.float16, 0, True),   # wide heads: prompts, one token
+    ([333], [333], 2, 2, 144, 16, "int8", torch.bfloat16, 100, True),
+    ([260, 40], [200, 45], 40, 1, 208, 128, "int8", torch.float16, 0, True),
+    ([515, 20], [129, 33], 3, 3, 160, 32, "e4m3", torch.bfloat16, 0, False),
+    ([2000], [130], 2, 2, 256, 128, "int8", torch.bfloat16, 0, True),         # wide heads, keys split among many CTAs
 ]
 
 
