@@ -27,7 +27,7 @@
 // of both tiles takes 4850 cycles, 2048 of them on the tensor pipe: what bounds it is the chain of one tile,
 // scores -> 430 cycles for the largest -> 2250 for the weights -> second product -> next scores.
 // Heads of 256, where nothing overlaps that chain: a prompt of 2048 tokens of 16 heads 130 us (653 in the rows
-// kernel), 509 tokens behind 8192, 16 over 4 heads, 166 us = 416 TFLOP/s (570 in the rows kernel).
+// kernel), 509 tokens behind 8192, 16 over 4 heads, 166 us = 424 TFLOP/s (570 in the rows kernel).
 //
 // Warps 0-3 and 4-7: softmax of a tile, a thread a row (the same warps fetch the queries and store the
 // outputs); 8-11: conversion; 12: issues the products; 13: copies; 14: scales of the pages; 15: the list of
