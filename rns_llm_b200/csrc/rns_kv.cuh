@@ -102,6 +102,12 @@ RNS_HD int kv_named(const KvView& c, int32_t page) {
 }
 RNS_HD int kv_page(const KvView& c, int b, int nth) { return kv_named(c, kv_entry(c, b, nth)); }
 
+// First key that a query at `position` sees.  A position before the first token sees nothing; it counts as the
+// first here, so that it less a window stays within 32 bits.
+RNS_HD int kv_first_key(const KvQuery& a, int position) {
+    return a.window > 0 ? (position > 0 ? position : 0) + 1 - a.window : 0;
+}
+
 #ifdef __CUDACC__
 template <typename T> __device__ __forceinline__ float kv_to_float(T v);
 template <> __device__ __forceinline__ float kv_to_float<__half>(__half v) { return __half2float(v); }

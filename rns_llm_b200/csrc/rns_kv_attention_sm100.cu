@@ -28,7 +28,8 @@ static int check_attention(const rns_kv_cache* cache, const rns_kv_attention_arg
     p->q = a->d_q; p->type = a->type; p->heads = a->heads; p->group = a->heads / c->kv_heads;
     p->tokens = a->tokens; p->q_token_stride = a->q_token_stride; p->q_head_stride = a->q_head_stride;
     p->lens = a->d_seq_lens; p->starts = a->d_query_starts;
-    p->causal = a->causal != 0; p->window = a->window;
+    // a window as long as the longest sequence there can be hides nothing
+    p->causal = a->causal != 0; p->window = a->window >= (int64_t)c->table_pages * c->page_tokens ? 0 : a->window;
     p->scale_log2 = a->softmax_scale * 1.4426950408889634f;
     p->out = a->d_out; p->out_token_stride = a->out_token_stride; p->out_head_stride = a->out_head_stride;
     p->lse = a->d_lse;

@@ -65,7 +65,7 @@ __device__ __forceinline__ void decode_range(const DecodeParams& p, DecodeItem& 
     const int t0 = it.tile / p.head_tiles * p.token_tile, t1 = min(t0 + p.token_tile, it.count);
     const int base = it.length - it.count;
     int last = p.a.causal ? base + t1 : it.length;
-    int first = p.a.window > 0 ? max(0, base + t0 - p.a.window + 1) : 0;
+    const int first = max(0, kv_first_key(p.a, base + t0));
     if (base + t1 <= 0) last = 0;
     it.key0 = first & ~(KEYS - 1);
     it.last = last;
@@ -399,8 +399,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // keys every row of the tile sees
         const int position = it.length - it.count + tile_t0;
         const int all_last = p.a.causal ? position + 1 : position >= 0 ? it.length : 0;
-        const int all_first = p.a.window > 0 ? position + n_tokens - p.a.window : 0;
-        const int tile_first = p.a.window > 0 ? position + 1 - p.a.window : 0;
+        const int all_first = kv_first_key(p.a, position + n_tokens - 1);
+        const int tile_first = kv_first_key(p.a, position);
 
         // and those that each of this thread's rows sees: [sees0, sees1)
         int sees0[NT][2], sees1[NT][2];
@@ -410,7 +410,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int e = 0; e < 2; ++e) {
                 const int pos = position + (nt * 8 + 2 * c4 + e) / p.head_tile;
                 sees1[nt][e] = pos < 0 ? 0 : p.a.causal ? pos + 1 : it.length;
-                sees0[nt][e] = p.a.window > 0 ? pos + 1 - p.a.window : 0;
+                sees0[nt][e] = kv_first_key(p.a, pos);
             }
 
         float o[MT][NT][4], m[NT][2], l[NT][2], v_unit = 0x1p-123f, per_unit = 0x1p123f;

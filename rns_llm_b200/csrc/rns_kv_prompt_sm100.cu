@@ -90,7 +90,7 @@ __device__ __forceinline__ void prompt_range(const PromptParams& p, PromptItem& 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int ta = it.token0 + i * p.token_tile, tb = min(ta + p.token_tile, it.count);
-        first[i] = p.a.window > 0 ? max(0, base + ta - p.a.window + 1) : 0;
+        first[i] = max(0, kv_first_key(p.a, base + ta));
         last[i] = p.a.causal ? base + tb : it.length;
         if (i >= p.tiles || ta >= it.count || base + tb <= 0) last[i] = 0;
         if (last[i] > first[i]) { low = min(low, first[i]); high = max(high, last[i]); }
@@ -601,11 +601,11 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int tok = it.token0 + tile * p.token_tile + row_token;
                 const int position = it.length - it.count + tok;
                 const int hi = position < 0 ? 0 : p.a.causal ? position + 1 : it.length;
-                const int lo = p.a.window > 0 ? position - p.a.window + 1 : 0;
+                const int lo = kv_first_key(p.a, position);
                 // keys that every row of the tile sees
                 const int tile_pos = it.length - it.count + it.token0 + tile * p.token_tile;
                 const int all_hi = p.a.causal ? tile_pos + 1 : tile_pos >= 0 ? it.length : 0;
-                const int all_lo = p.a.window > 0 ? tile_pos + p.token_tile - p.a.window : 0;
+                const int all_lo = kv_first_key(p.a, tile_pos + p.token_tile - 1);
                 float m = kNoScore, l = 0.0f, unit = 0.0f;
                 for (int j = part.live0; j < live1; ++j) {
                     const int slot = scale_uses % kScaleSlots;
