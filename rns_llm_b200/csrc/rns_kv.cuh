@@ -156,6 +156,28 @@ template <int FORMAT> __device__ __forceinline__ void kv_decode4(uint32_t w, flo
         }
     }
 }
+// A page's value scale s as 2^exponent * weight, and 2^-exponent.  Attention keeps a row's softmax weights in
+// units of 2^M, where M is a whole number near the largest (score + exponent) that the row has met:
+//     w_j = 2^(t_j + exponent - M) * weight          what is rounded to fp16 and meets the bytes
+//     l   = sum 2^(t_j + exponent - M) * 2^-exponent the softmax's sum, fp32
+// so fp16's range lies where the row's own contributions are, whatever the scales of pages that it does not
+// see or heed (a unit near the largest scale met lost the other pages: a scale 2^14 above theirs cost 5 % of
+// an output, one 2^26 above all of it).  M - exponent is a difference of whole numbers, exact.  The exponent is
+// kept within [-64, 126]: its powers of two are normal numbers and l does not overflow; smaller scales (zeros
+// among them) have weights below one.  l loses terms only where scales within a row differ by more than 2^100.
+// A scale that is not finite has weight NaN, which reaches the rows that see it.
+struct KvValueScale {
+    float exponent, weight, back;
+};
+__device__ __forceinline__ KvValueScale kv_value_scale(float s) {
+    const bool finite = fabsf(s) <= 3.0e38f;
+    const int e = finite ? max(63, min(253, (int)(__float_as_uint(s) >> 23 & 255u))) : 127;
+    KvValueScale v;
+    v.back = __uint_as_float((uint32_t)(254 - e) << 23);
+    v.weight = finite ? s * v.back : __uint_as_float(0x7fc00000u);
+    v.exponent = __uint_as_float(0x4B000000u + (uint32_t)e) - (8388608.0f + 127.0f);
+    return v;
+}
 // x / scale on the grid, eight values -> bytes; inverse = 1 / scale.  The quotient is the correctly rounded
 // one: the product with the inverse is off by at most two units in the last place, so only values that
 // close to the middle between two grid points need the division.

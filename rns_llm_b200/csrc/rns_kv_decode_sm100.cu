@@ -19,14 +19,14 @@
 //   subtraction, exact; e4m3 with the conversion instruction, exact - in whatever order of the inner
 //   index costs least: sums do not depend on it, and Q is laid out to match.
 // * Queries are scaled by a power of two per row into fp16's range, exact for bf16 as well up to
-//   2^-32 of the row's largest element.  Scores, the softmax and all sums are fp32.  Each weight is
-//   rounded to fp16 (2^-11) for the second product, in units of a power of two near the largest value
-//   scale met so far, so that a page's scale is part of the weight and the accumulators need no scale
-//   of their own.
-// * The running maximum may lag by 2^8 (a value scale by 2^4): then weights exceed one but nothing
-//   is lost, and the accumulators are rescaled only when a vote finds a larger score.  The maximum of
-//   a row follows that row's scores alone, and units are powers of two: but for weights below fp16's
-//   normal range, what a row gives does not depend on the rows beside it.
+//   2^-32 of the row's largest element.  Scores, the softmax and all sums are fp32.  Each weight, with
+//   its page's value scale, is rounded to fp16 (2^-11) for the second product, in units of a power of
+//   two near the row's largest such weight (kv_value_scale); the accumulators need no scale of their
+//   own.  Weights 2^14 below that are off by up to 2^-25 of the unit each.
+// * The running maximum may lag by 2^8: then weights exceed one but nothing is lost, and the
+//   accumulators are rescaled only when a vote finds a larger score.  It is a whole number, so that
+//   rescaling is exact, and follows the row's own scores and their pages' scales alone: what a row
+//   gives does not depend on the rows beside it.
 //
 // Measured (graph replay): 64 sequences of 1..8192 tokens, 32 over 8 heads of 128, 143 us = 3.75 TB/s of cache
 // (0.58 of the copy rate; 450 instructions for 16 keys, issue slots 53 % busy with three warps a scheduler: the
@@ -413,7 +413,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 sees0[nt][e] = kv_first_key(p.a, pos);
             }
 
-        float o[MT][NT][4], m[NT][2], l[NT][2], v_unit = 0x1p-123f, per_unit = 0x1p123f;
+        float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -436,8 +436,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         if (k0 >= it.last) break;
                         if (k0 + 16 <= tile_first) continue;
                         const float k_scale = my_scales[slot * 4 + half];
-                        float v_scale = my_scales[slot * 4 + 2 + half];
-                        if (!(fabsf(v_scale) <= 3.0e38f)) v_scale = __uint_as_float(0x7fc00000u);
+                        const KvValueScale vs = kv_value_scale(my_scales[slot * 4 + 2 + half]);
                         // two chains of products for each tile, so that they do not wait for one another
                         float s[NT][4], s2[NT][4];
 #pragma unroll
@@ -466,7 +465,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                             }
                         }
                         const bool whole = k0 + 16 <= all_last && k0 >= all_first;
-                        bool grow = fabsf(v_scale) > 16.0f * v_unit;
+                        bool grow = false;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -484,15 +483,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) grow = grow || s[nt][e] > m[nt][e & 1] + kLag;
+                            for (int e = 0; e < 4; ++e) grow = grow || s[nt][e] > m[nt][e & 1] - vs.exponent + kLag;
                         if (__any_sync(0xffffffffu, grow)) {
-                            float v_ratio = 1.0f;
-                            if (fabsf(v_scale) > 16.0f * v_unit) {
-                                const float unit = __uint_as_float(__float_as_uint(v_scale) & 0x7f800000u);
-                                v_ratio = v_unit / unit;
-                                v_unit = unit;
-                                per_unit = 1.0f / unit;                                // a power of two: exact
-                            }
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -500,24 +492,23 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                     float top = fmaxf(s[nt][e], s[nt][e + 2]);
 #pragma unroll
                                     for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                                    if (!(top > m[nt][e] + kLag)) top = m[nt][e];  // a row's result is its own affair
+                                    top = top > m[nt][e] - vs.exponent + kLag ? ceilf(top + vs.exponent) : m[nt][e];  // a row's result is its own affair
                                     const float keep = exp2_approx(m[nt][e] - top);
                                     m[nt][e] = top;
                                     l[nt][e] *= keep;
 #pragma unroll
-                                    for (int i = 0; i < MT; ++i) { o[i][nt][e] *= keep * v_ratio; o[i][nt][e + 2] *= keep * v_ratio; }
+                                    for (int i = 0; i < MT; ++i) { o[i][nt][e] *= keep; o[i][nt][e + 2] *= keep; }
                                 }
                         }
-                        const float weight = v_scale * per_unit;
                         uint32_t pf[NT][2];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float w[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float pe = exp2_approx(s[nt][e] - m[nt][e & 1]);
-                                l[nt][e & 1] += pe;
-                                w[e] = pe * weight;
+                                const float pe = exp2_approx(s[nt][e] - (m[nt][e & 1] - vs.exponent));
+                                l[nt][e & 1] = fmaf(pe, vs.back, l[nt][e & 1]);
+                                w[e] = pe * vs.weight;
                                 if (!whole && s[nt][e] == -INFINITY) w[e] = 0.0f;      // not NaN from the page's scale
                             }
                             const __half2 top = __floats2half2_rn(w[0], w[1]), low = __floats2half2_rn(w[2], w[3]);
@@ -589,7 +580,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 float top = kNoMax;
 #pragma unroll
                 for (int w = 0; w < kDecodeWarps; ++w) top = fmaxf(top, warp_m[w * ROWS + nt * 8 + 2 * c4 + e]);
-                factor[nt][e] = exp2_approx(m[nt][e] - top) * v_unit;
+                factor[nt][e] = exp2_approx(m[nt][e] - top);
             }
 #pragma unroll 1
         for (int w = 0; w < kDecodeWarps; ++w) {

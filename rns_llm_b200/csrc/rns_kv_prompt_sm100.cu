@@ -3,7 +3,7 @@
 // A CTA works on two tiles of 128 query rows of one head of the cache (tokens x the heads that share
 // it) and walks the keys in blocks of 128.  Per block and tile:
 //     S = Q K^T          tcgen05, both operands fp16 in shared memory, S fp32 in tensor memory
-//     P = 2^(S f - m) w  one thread per row: S from tensor memory, P back into its place as fp16
+//     P = 2^(S f - M) w  one thread per row: S from tensor memory, P back into its place as fp16
 //     O += P V           tcgen05, P from tensor memory, V fp16 in shared memory, O in tensor memory
 // The bound is the tensor pipe (4 * 128 * 128 * head_dim operations a block and tile), with the
 // exponentials (16 a clock and SM) close behind; bytes from memory hardly count, since a block serves
@@ -17,8 +17,9 @@
 //   is stored).  The same tile layout - 64 dimensions x 128 keys - is K-major for the first product
 //   and MN-major for the second, so V needs no transposition.
 // * Numerics are those of the rows kernel: queries times a power of two per row, fp32 scores, softmax
-//   and sums, weights rounded to fp16 in units of a power of two near the largest value scale; the
-//   running maximum may lag by 2^8, so that O in tensor memory is rescaled only now and then.
+//   and sums, weights with their pages' value scales rounded to fp16 in units of a power of two near the
+//   row's largest; the running maximum may lag by 2^8, so that O in tensor memory is rescaled only now
+//   and then.
 // * Work is cut as there: one axis of key blocks over all items, equal shares, pieces joined by a
 //   second kernel.
 //
@@ -70,7 +71,7 @@ struct PromptItem {
     int64_t begin;
     int count, length;
     int token0, head0;                    // first token of the pair inside the sequence, first head of its head tile
-    int low, key0, blocks;                // first key that any row sees, rounded down to a block
+    int key0, blocks;                     // first key that any row sees, rounded down to a block
     int from[2], to[2];                   // blocks that a tile needs
 };
 
@@ -95,7 +96,6 @@ __device__ __forceinline__ void prompt_range(const PromptParams& p, PromptItem& 
         if (i >= p.tiles || ta >= it.count || base + tb <= 0) last[i] = 0;
         if (last[i] > first[i]) { low = min(low, first[i]); high = max(high, last[i]); }
     }
-    it.low = low;
     it.key0 = high > 0 ? low & ~(kBlock - 1) : 0;
     it.blocks = high > 0 ? (high - it.key0 + kBlock - 1) / kBlock : 1;    // nothing to see: zeros to write
 #pragma unroll
@@ -306,9 +306,7 @@ struct PromptBars {
     uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots], part_full[kPartSlots], part_empty[kPartSlots];
 };
 struct PromptScales {
-    float key[8], weight[8];              // of 16 keys each: key scale, value scale / unit
-    float unit, ratio;                    // this block's unit; the previous unit / this one
-    float pad[2];
+    float key[8], exponent[8], weight[8], back[8];   // of 16 keys each: key scale, and the value scale's kv_value_scale
 };
 
 // Bits [lo, hi) of the 32 columns from `at` on: those a row sees.
@@ -316,7 +314,7 @@ __device__ __forceinline__ uint32_t prompt_seen(int at, int lo, int hi) {
     const int a = min(max(lo - at, 0), 32), b = min(max(hi - at, 0), 32);
     return (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
 }
-// The largest score of a row of a block, of which it sees every column.
+// The largest score, with its page's value exponent, of a row of a block of which it sees every column.
 __device__ __forceinline__ float prompt_top(uint32_t s_tmem, const PromptScales& sc, float q_scale) {
     float s[kBlock];
 #pragma unroll
@@ -332,16 +330,15 @@ __device__ __forceinline__ float prompt_top(uint32_t s_tmem, const PromptScales&
             b = max3(b, s[g * 16 + i + 2], s[g * 16 + i + 3]);
         }
         a = max3(a, s[g * 16 + 14], s[g * 16 + 15]);
-        top = fmaxf(top, fmaxf(a, b) * (sc.key[g] * q_scale));
+        top = fmaxf(top, fmaf(fmaxf(a, b), sc.key[g] * q_scale, sc.exponent[g]));
     }
     return top;
 }
-// Scores -> weights 2^(s f - m), whose sum is returned, and times the values' scale as fp16 into the place of the
-// scores.  A loop over 32 columns, read a second time, rather than 128 held and unrolled: the code of all
+// Scores -> 2^(s f + exponent - m), whose sum without the exponents is returned, and times the values' weight as
+// fp16 into the place of the scores.  A loop over 32 columns, read a second time, rather than 128 held and unrolled: the code of all
 // eight programs has to stay in the instruction caches.  The next columns are fetched as soon as the
 // multiply-adds have taken these.
 __device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const PromptScales& sc, float q_scale, float m) {
-    const Pair minus_m = pair(-m, -m);
     Pair sums[4] = {0, 0, 0, 0};                                    // independent: the additions must not wait for one another
     float s[32];
     tmem_ld32(s_tmem, s);
@@ -349,17 +346,18 @@ __device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const PromptSca
     for (int ch = 0; ch < 4; ++ch) {
         Pair e[16];
         const float f0 = sc.key[ch * 2] * q_scale, f1 = sc.key[ch * 2 + 1] * q_scale;
-        const float w0 = sc.weight[ch * 2], w1 = sc.weight[ch * 2 + 1];
+        const float c0 = sc.exponent[ch * 2] - m, c1 = sc.exponent[ch * 2 + 1] - m;
+        const float w0 = sc.weight[ch * 2], w1 = sc.weight[ch * 2 + 1], b0 = sc.back[ch * 2], b1 = sc.back[ch * 2 + 1];
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            e[i] = fma2(pair(s[2 * i], s[2 * i + 1]), i < 8 ? pair(f0, f0) : pair(f1, f1), minus_m);
+            e[i] = fma2(pair(s[2 * i], s[2 * i + 1]), i < 8 ? pair(f0, f0) : pair(f1, f1), i < 8 ? pair(c0, c0) : pair(c1, c1));
         tmem_ld32(s_tmem + (ch < 3 ? ch + 1 : 3) * 32, s);          // (the last time to no purpose: its columns are not written yet)
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             e[i] = pair(prompt_exp2(pair_x(e[i])), prompt_exp2(pair_y(e[i])));
-            sums[i & 3] = add2(sums[i & 3], e[i]);
+            sums[i & 3] = fma2(e[i], i < 8 ? pair(b0, b0) : pair(b1, b1), sums[i & 3]);
             const Pair pw = mul2(e[i], i < 8 ? pair(w0, w0) : pair(w1, w1));
             const __half2 h = __floats2half2_rn(pair_x(pw), pair_y(pw));
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
@@ -383,7 +381,7 @@ __device__ __forceinline__ float prompt_top_seen(uint32_t s_tmem, const PromptSc
         float best = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) best = fmaxf(best, (seen >> i) & 1 ? s[i] : -INFINITY);
-        top = fmaxf(top, best * (sc.key[g] * q_scale));
+        top = fmaxf(top, fmaf(best, sc.key[g] * q_scale, sc.exponent[g]));
     }
     return top;
 }
@@ -395,14 +393,14 @@ __device__ __forceinline__ float prompt_weights_seen(uint32_t s_tmem, const Prom
         tmem_ld16(s_tmem + g * 16, s);
         tmem_ld_wait();
         const uint32_t seen = prompt_seen(g * 16, lo, hi);
-        const float f = sc.key[g] * q_scale, weight = sc.weight[g];
+        const float f = sc.key[g] * q_scale, c = sc.exponent[g] - m, weight = sc.weight[g], back = sc.back[g];
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             // zero where the row does not see, not NaN from a scale that it does not see
             const bool a = (seen >> i) & 1, b = (seen >> (i + 1)) & 1;
-            const float e0 = a ? prompt_exp2(fmaf(s[i], f, -m)) : 0.0f, e1 = b ? prompt_exp2(fmaf(s[i + 1], f, -m)) : 0.0f;
-            sum += e0 + e1;
+            const float e0 = a ? prompt_exp2(fmaf(s[i], f, c)) : 0.0f, e1 = b ? prompt_exp2(fmaf(s[i + 1], f, c)) : 0.0f;
+            sum = fmaf(e0 + e1, back, sum);
             const __half2 h = __floats2half2_rn(a ? e0 * weight : 0.0f, b ? e1 * weight : 0.0f);
             w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
         }
@@ -606,7 +604,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int tile_pos = it.length - it.count + it.token0 + tile * p.token_tile;
                 const int all_hi = p.a.causal ? tile_pos + 1 : tile_pos >= 0 ? it.length : 0;
                 const int all_lo = kv_first_key(p.a, tile_pos + p.token_tile - 1);
-                float m = kNoScore, l = 0.0f, unit = 0.0f;
+                float m = kNoScore, l = 0.0f;
                 for (int j = part.live0; j < live1; ++j) {
                     const int slot = scale_uses % kScaleSlots;
                     ok = prompt_wait(smem_addr(&bars.scale_full[slot]), (scale_uses / kScaleSlots) & 1, abort, wait_code(1, slot));
@@ -617,8 +615,6 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         continue;
                     }
                     const PromptScales& sc = scales[slot];
-                    const float ratio = sc.ratio;
-                    unit = sc.unit;
                     ok = prompt_wait(smem_addr(&bars.s_full[tile]), blocks_seen & 1, abort, wait_code(2, tile));
                     if (!ok) break;
                     ++blocks_seen;
@@ -626,9 +622,9 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     const int key = key0 + j * kBlock;
                     const bool whole = key + kBlock <= all_hi && key >= all_lo;
                     float top = whole ? prompt_top(s_tmem, sc, q_scale) : prompt_top_seen(s_tmem, sc, q_scale, lo - key, hi - key);
-                    if (__any_sync(0xffffffffu, top > m + kScoreLag || ratio != 1.0f)) {
-                        if (!(top > m + kScoreLag)) top = m;
-                        const float keep = prompt_exp2(m - top), change = keep * ratio;
+                    if (__any_sync(0xffffffffu, top > m + kScoreLag)) {
+                        top = top > m + kScoreLag ? ceilf(top) : m;
+                        const float keep = prompt_exp2(m - top);
                         m = top;
                         l *= keep;
                         // S(j) has arrived, so the product of the block before has: O is at rest
@@ -640,7 +636,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                 tmem_ld8f(o_tmem + ch * 8, o);
                                 tmem_ld_wait();
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[i] * change);
+                                for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[i] * keep);
                                 tmem_st8(o_tmem + ch * 8, v);
                             }
                         }
@@ -682,7 +678,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const bool none = part.stop == part.step;
                 float* piece = p.partial + ((int64_t)blockIdx.x * 2 + part.slot) * S::kPartial;
                 const int at = tile * kTileRows + row;
-                const float factor = complete ? (empty ? 0.0f : unit / l) : unit;
+                const float factor = complete ? (empty ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll 1
                 for (int d = 0; d < DIM && !none; d += 16) {
                     float o[16];
@@ -930,8 +926,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const PromptPart& part = parts[n_part % kPartSlots];
                 more = !part.last;
                 const int live1 = part.live1, b = part.it.b, kv_head = part.it.kv_head, key0 = part.it.key0;
-                const int length = part.it.length, low = part.it.low;
-                float unit = 0x1p-123f;
+                const int length = part.it.length;
                 // four blocks at a time, as the copies: a lane for 16 keys
                 const int live0 = part.live0, mine = lane >> 3;
                 const auto entry = [&](int at) {
@@ -952,24 +947,19 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         }
                     }
                     next = entry(j0 + 4);
-                    if (!(fabsf(vs) <= 3.0e38f)) vs = __uint_as_float(0x7fc00000u);
-                    // the largest of the finite ones that some row sees
-                    const uint32_t size = vs == vs && key + 16 > low ? __float_as_uint(fabsf(vs)) : 0u;
+                    const KvValueScale value = kv_value_scale(vs);
 #pragma unroll 1
                     for (int i = 0; i < 4 && j0 + i < live1; ++i) {
-                        const uint32_t top = __reduce_max_sync(0xffffffffu, mine == i ? size : 0u);
-                        float ratio = 1.0f;
-                        if (__uint_as_float(top) > 16.0f * unit) {
-                            const float grown = __uint_as_float(top & 0x7f800000u);
-                            ratio = unit / grown;
-                            unit = grown;
-                        }
                         const int slot = n % kScaleSlots;
                         ok = prompt_wait(smem_addr(&bars.scale_empty[slot]), ((n / kScaleSlots) & 1) ^ 1, abort, wait_code(12, slot));
                         if (!ok) break;
                         ++n;
-                        if (mine == i) { scales[slot].key[lane & 7] = ks; scales[slot].weight[lane & 7] = vs / unit; }
-                        if (lane == 0) { scales[slot].unit = unit; scales[slot].ratio = ratio; }
+                        if (mine == i) {
+                            scales[slot].key[lane & 7] = ks;
+                            scales[slot].exponent[lane & 7] = value.exponent;
+                            scales[slot].weight[lane & 7] = value.weight;
+                            scales[slot].back[lane & 7] = value.back;
+                        }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_addr(&bars.scale_full[slot]));
                     }

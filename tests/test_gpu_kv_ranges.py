@@ -1,10 +1,18 @@
-"""The quantised key/value cache at the ends of its ranges, on the GPU: windows near 2^31 first.
+"""The quantised key/value cache at the ends of its ranges, on the GPU: windows, scales of very different
+size, values that are not finite, bounds and positions at their limits.
+
+Attention is compared with float64 element by element.  Its bound is that of test_gpu_kv_cache.py but for the
+weights below fp16's normal range: a weight is rounded in units of 2^M, where 2^M is at most twice the largest
+p_j * scale_j over the keys that THE ROW SEES (p_j: its softmax weight, scale_j: the value scale of the key's
+page), by up to half of fp16's smallest step, 2^-25.  It meets a byte of at most Q (127 or 448) there, so a row
+of n keys is off by n * 2^-24 * max_j (p_j * scale_j * Q), whatever pages it does not see or heed hold.
 """
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv_cache import Setup, check_attention, starts_of
+import kv_oracle as O
+from test_gpu_kv_cache import ATTENTION, HALF_STEP, Setup, check_attention, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +46,166 @@ def test_wide_window_with_more_queries_than_tokens(backend, lens, new, heads, wi
                                                   max_query_len=max(new), return_lse=True)
     assert torch.equal(got, plain) and torch.equal(lse, plain_lse)
     backend.check_status()
+
+
+# ---------------------------------------------------------------------------------------
+# value scales
+# ---------------------------------------------------------------------------------------
+SMALLEST = {torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}      # of the output types
+
+
+def check_rows(s, q, new, got, lse, *, scale, dtype, causal=True, window=0, telling=None):
+    """Outputs and lse against float64 by the bound above; `telling`: the share of outputs that the bound must
+    be able to tell from zero ten times over."""
+    starts, (_, heads, dim) = starts_of(new), q.shape
+    got = got.float().cpu().numpy().astype(np.float64)
+    lse = lse.cpu().numpy().astype(np.float64)
+    told = []
+    for b, n in enumerate(new):
+        keys, values = s.values(b, 0), s.values(b, 1)
+        rows = slice(starts[b], starts[b + 1])
+        x = q[rows].float().numpy()
+        want, want_lse, spread, loud = O.attention(x, keys, values, s.lens[b], scale=scale, causal=causal, window=window)
+        group = heads // keys.shape[1]
+        holds = np.stack([s.scale[1][s.table[b][t // s.page]] for t in range(s.lens[b])]) if s.lens[b] else None
+        most = np.zeros((n, heads))                              # n_keys * max_j p_j scale_j Q of each row
+        for i in range(n):
+            position = s.lens[b] - n + i
+            if position < 0:
+                continue
+            first, last = max(0, position - window + 1) if window else 0, position + 1 if causal else s.lens[b]
+            for h in range(heads):
+                t = keys[first:last, h // group].astype(np.float64) @ x[i, h].astype(np.float64) * scale
+                p = np.exp(t - want_lse[i, h])
+                most[i, h] = (last - first) * (p * holds[first:last, h // group]).max() * float(O.LARGEST[s.fmt])
+        score = (dim + 8) * 2.0 ** -22 * loud[:, :, None]
+        bound = (HALF_STEP[dtype] * np.abs(want) + (2.0 ** -11 + 2.0 ** -20 + 2 * score) * spread * 1.01 +
+                 2.0 ** -24 * 1.01 * most[:, :, None] + SMALLEST[dtype])
+        error = np.abs(got[rows] - want)
+        assert np.isfinite(got[rows]).all()
+        assert (error <= bound).all(), (b, float((error / bound).max()))
+        told.append((bound * 10 < np.abs(want)).ravel())
+        slack = (dim + 8) * 2.0 ** -22 * loud + 2.0 ** -20 * (1 + np.abs(np.where(np.isinf(want_lse), 0, want_lse)))
+        seen = ~np.isneginf(want_lse)
+        assert np.array_equal(np.isneginf(lse[rows]), ~seen)
+        assert (np.abs(lse[rows][seen] - want_lse[seen]) <= slack[seen]).all()
+    if telling is not None:
+        assert np.concatenate(told).mean() >= telling, np.concatenate(told).mean()
+
+
+def attend(backend, s, q, new, **kw):
+    return backend.kv_cache_attention(q.cuda(), s.cache, s.d_table, s.ints(s.lens), s.ints(starts_of(new)),
+                                      max_query_len=max(new), return_lse=True, **kw)
+
+
+@pytest.mark.parametrize("lens,new,heads,kv_heads,dim,page,fmt,dtype,window,causal", ATTENTION)
+def test_error_is_relative_to_what_a_row_sees(backend, lens, new, heads, kv_heads, dim, page, fmt, dtype, window, causal):
+    s = Setup(backend, lens, kv_heads=kv_heads, dim=dim, page=page, fmt=fmt, seed=heads * dim + sum(lens) + 1)
+    q = queries(s, sum(new), heads, dim, dtype)
+    got, lse = attend(backend, s, q, new, window=window or None, causal=causal)
+    check_rows(s, q, new, got, lse, scale=dim ** -0.5, dtype=dtype, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("spread", [1.0, 4.0])
+@pytest.mark.parametrize("gain", [1.0, 20.0])
+def test_pages_of_all_sizes(backend, new, spread, gain):
+    """Value scales over up to 46 powers of two, key scales as they are in a model."""
+    lens = [400, 90]
+    s = Setup(backend, lens, kv_heads=2, dim=64, page=16, seed=int(gain) + int(spread), spread=spread)
+    for scale in s.scale[0]:
+        scale[:] = 1 / float(O.LARGEST["int8"])
+    s.to_device()
+    q = torch.from_numpy((s.rng.standard_normal((2 * new, 4, 64)) * gain).astype(np.float32)).bfloat16()
+    got, lse = attend(backend, s, q, [new, new])
+    check_rows(s, q, [new, new], got, lse, scale=0.125, dtype=torch.bfloat16, telling=0.5)
+
+
+def with_outlier(backend, fmt, dim, page, where, seed, lens=(400, 90)):
+    """Keys so that page `where` of sequence 0 has scores near -70 and the others a spread of 2, for queries
+    near the vector that is returned."""
+    s = Setup(backend, list(lens), kv_heads=2, dim=dim, page=page, fmt=fmt, seed=seed)
+    top = float(O.LARGEST[fmt])
+    toward = np.where(s.rng.random(dim) < 0.5, -1.0, 1.0).astype(np.float32)
+    s.scale[0][:] = 2 / (top / 3)
+    page_id = s.table[0, where]
+    s.data[0][page_id] = O.to_bytes(np.broadcast_to(-top * toward, s.data[0][page_id].shape).copy(), fmt)
+    s.scale[0][page_id] = 70 / (top * dim ** 0.5)
+    return s, page_id, toward
+
+
+def near(s, toward, tokens, heads, dtype):
+    noise = s.rng.standard_normal((tokens, heads, len(toward))).astype(np.float32)
+    return torch.from_numpy(toward + 0.2 * noise).to(dtype)
+
+
+@pytest.mark.parametrize("new", [1, 5, 70])
+@pytest.mark.parametrize("power", [10, 14, 20, 30, 60])
+@pytest.mark.parametrize("fmt,dim,where", [("int8", 64, 0), ("int8", 128, 3), ("e4m3", 80, 24), ("e4m3", 256, 1)])
+def test_page_of_large_values_that_no_row_heeds(backend, fmt, dim, where, power, new):
+    """A page whose values are 2^power larger and whose softmax weight is e^-70: the other pages keep their
+    precision."""
+    s, page_id, toward = with_outlier(backend, fmt, dim, 16, where, seed=power + dim)
+    s.scale[1][page_id] *= np.float32(2.0 ** power)
+    s.to_device()
+    q = near(s, toward, 2 * new, 4, torch.float16)
+    got, lse = attend(backend, s, q, [new, new])
+    check_rows(s, q, [new, new], got, lse, scale=dim ** -0.5, dtype=torch.float16, telling=0.5)
+
+
+@pytest.mark.parametrize("power", [14, 30])
+def test_page_of_large_values_among_many_long_sequences(backend, power):
+    """The same where a warp of the rows kernel meets many pages of one row."""
+    lens = [2100] * 16
+    s = Setup(backend, lens, kv_heads=8, dim=64, page=64, seed=power)
+    top = 127.0
+    toward = np.where(s.rng.random(64) < 0.5, -1.0, 1.0).astype(np.float32)
+    s.scale[0][:] = 2 / (top / 3)
+    large = s.table[:, 1]                                        # in every sequence
+    s.data[0][large] = (-top * toward).astype(np.int8)
+    s.scale[0][large] = 70 / (top * 8)
+    s.scale[1][large] *= np.float32(2.0 ** power)
+    s.to_device()
+    q = near(s, toward, 16, 8, torch.float16)
+    got, lse = attend(backend, s, q, [1] * 16)
+    check_rows(s, q, [1] * 16, got, lse, scale=0.125, dtype=torch.float16, telling=0.5)
+
+
+@pytest.mark.parametrize("new", [4, 90])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_later_page_of_large_values(backend, dim, new):
+    """What a row gives does not depend on the value scale of a page that it does not see."""
+    lens = [146]
+    s = Setup(backend, lens, kv_heads=1, dim=dim, page=16, seed=dim)
+    q = queries(s, new, 4, dim)
+    clean, _ = attend(backend, s, q, [new])
+    s.scale[1][s.table[0, 9]] *= np.float32(2.0 ** 40)           # positions 144, 145
+    s.to_device()
+    got, lse = attend(backend, s, q, [new])
+    assert torch.equal(got[:new - 2], clean[:new - 2])
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("power", [-60, -20, 0, 60, 110])
+def test_scales_near_the_ends_of_their_type(backend, power, new):
+    lens = [400, 90]
+    s = Setup(backend, lens, kv_heads=2, dim=64, page=16, seed=power + 100)
+    s.scale[1] *= np.float32(2.0 ** power)
+    s.to_device()
+    q = queries(s, 2 * new, 4, 64, torch.bfloat16)
+    got, lse = attend(backend, s, q, [new, new])
+    check_rows(s, q, [new, new], got, lse, scale=0.125, dtype=torch.bfloat16, telling=0.3)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_pages_of_zeros(backend, new):
+    """Value scales of zero on every page of one sequence and on some of the other's."""
+    lens = [400, 90]
+    s = Setup(backend, lens, kv_heads=2, dim=64, page=16, seed=41)
+    s.scale[1][s.table[1, :6]] = 0
+    s.scale[1][s.table[0, 1:20]] = 0
+    s.to_device()
+    q = queries(s, 2 * new, 4, 64)
+    got, lse = attend(backend, s, q, [new, new])
+    check_rows(s, q, [new, new], got, lse, scale=0.125, dtype=torch.float16)
+    assert (got[new:] == 0).all()
