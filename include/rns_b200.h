@@ -564,6 +564,9 @@ typedef enum rns_kv_format {
  *                         beyond a sequence's length are not read.
  *   d_status              int32 [1] or NULL
  * page_tokens: 16, 32, 64 or 128; head_dim: a multiple of 16 up to 256.
+ * The bytes of a sequence's tokens are numbers: e4m3's two NaN patterns do not stand among them
+ * (rns_kv_write writes none; one that a caller puts there makes rows NaN that do not see it).  A
+ * scale may be NaN, which reaches the rows that see its page and no others.
  *
  * Lengths, starts and page indices are read on the device.  One that is out of range sets
  * *d_status = RNS_ERR_BAD_INDEX and touches no memory: a sequence with a bad length or start
@@ -603,7 +606,7 @@ RNS_API int rns_host_kv_rows(const rns_kv_cache* cache, const int32_t* seq_lens,
  *   s = max(max |x|, eps) / Q, at least the old scale where the block holds earlier tokens;
  *   earlier tokens become round(q * (s_old / s)), new ones round(x / s), ties to even, clamped;
  * eps = 2^-23, Q = 127 (int8) or 448 (e4m3).  A block that is given an infinity or NaN gets the
- * scale NaN.  max_new: no sequence of the call has more new tokens (one that does is flagged
+ * scale NaN and bytes of zero, also by later writes to it.  max_new: no sequence of the call has more new tokens (one that does is flagged
  * and not written).  Rows of a block beyond the sequence's length stay as they are.
  */
 RNS_API int rns_kv_write(const rns_kv_cache* cache, const void* d_k_new, const void* d_v_new,

@@ -179,11 +179,16 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VECTOR ? 1024 / THR
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) top = max(top, warp_top[w]);
     // Bit patterns of magnitudes order like the numbers, with infinities and NaN on top: a block
-    // that was given one gets the scale NaN, so that it never reads back as something else.
+    // that was given one gets the scale NaN, so that it never reads back as something else, and bytes of zero:
+    // attention multiplies the bytes that a row does not see by zero, which removes no NaN.
     float s_new = __fdiv_rn(fmaxf(__uint_as_float(top), kKvEps), FORMAT == RNS_KV_INT8 ? 127.0f : 448.0f);
     if (top >= 0x7f800000u || old_scale != old_scale) s_new = __uint_as_float(0x7fc00000u);
     else s_new = fmaxf(s_new, old_scale);
     if (t == 0) *scale = s_new;
+    if (s_new != s_new) {
+        for (int g = t; g < last; g += THREADS) *reinterpret_cast<uint2*>(data + (int64_t)g * 8) = make_uint2(0, 0);
+        return;
+    }
     if (row0 > 0 && s_new != old_scale) {                          // the scale grew: the tokens that stay follow
         const float ratio = __fdiv_rn(old_scale, s_new);
         uint32_t* words = reinterpret_cast<uint32_t*>(data);

@@ -209,3 +209,68 @@ def test_pages_of_zeros(backend, new):
     got, lse = attend(backend, s, q, [new, new])
     check_rows(s, q, [new, new], got, lse, scale=0.125, dtype=torch.float16)
     assert (got[new:] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------
+# values that are not finite
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_bytes_of_a_block_with_a_value_that_is_not_finite(backend, fmt, bad, dtype):
+    """Scale NaN and bytes of zero, its earlier tokens' and later ones' too; every other block, scale and
+    byte as the NumPy statement has it."""
+    s = Setup(backend, [40, 20], fmt=fmt, seed=9)
+    x = s.rng.standard_normal((12, 2, 64)).astype(np.float32)
+    x = torch.from_numpy(x).to(dtype)
+    lens, starts = [40, 20], [0, 8, 12]                          # positions 32 .. 39 and 16 .. 19
+    x[3, 1, 7] = bad
+    with np.errstate(invalid="ignore"):
+        for which in range(2):
+            O.write(s.data[which], s.scale[which], x.float().numpy(), s.table, lens, starts, fmt)
+            s.data[which][s.table[0, 2], 1, :8] = 0
+    backend.kv_cache_write(s.cache, x.cuda(), x.cuda(), s.d_table, s.ints(lens), s.ints(starts))
+    s.check_bytes()
+    y = torch.ones(1, 2, 64, dtype=dtype)                        # one more token for that page
+    with np.errstate(invalid="ignore"):
+        for which in range(2):
+            O.write(s.data[which], s.scale[which], y.float().numpy(), s.table, [41], [0, 1], fmt)
+            s.data[which][s.table[0, 2], 1, :9] = 0
+    backend.kv_cache_write(s.cache, y.cuda(), y.cuda(), s.d_table[:1], s.ints([41]), s.ints([0, 1]))
+    s.check_bytes()
+    # a page that held tokens before
+    z = torch.full((1, 2, 64), bad, dtype=dtype)
+    with np.errstate(invalid="ignore"):
+        for which in range(2):
+            O.write(s.data[which], s.scale[which], z.float().numpy(), s.table[1:], [21 - 16], [0, 1], fmt)
+            s.data[which][s.table[1, 0], :, :5] = 0
+    backend.kv_cache_write(s.cache, z.cuda(), z.cuda(), s.d_table[1:], s.ints([5]), s.ints([0, 1]))
+    s.check_bytes()
+    backend.check_status()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("length,new,at", [(40, 40, 35), (18, 4, 16), (300, 150, 290)])
+def test_written_infinity_reaches_the_rows_that_see_it(backend, fmt, dim, length, new, at):
+    """A value that is not finite is written among a prompt's: rows that see its page of 16 tokens are NaN, the
+    others what they are without it."""
+    gen = torch.Generator().manual_seed(dim)
+    x = torch.randn(length, 1, dim, generator=gen).half()
+    q = torch.randn(new, 2, dim, generator=gen).half().cuda()
+    outs = []
+    for bad in (None, float("inf"), float("nan")):
+        v = x.clone()
+        if bad is not None:
+            v[at, 0, 5] = bad
+        cache = backend.create_kv_cache(pages=-(-length // 16), kv_heads=1, head_dim=dim, page_tokens=16, format=fmt)
+        table = torch.arange(cache.pages, dtype=torch.int32, device="cuda").view(1, -1)
+        ints = lambda *n: torch.tensor(n, dtype=torch.int32, device="cuda")
+        backend.kv_cache_write(cache, x.cuda(), v.cuda(), table, ints(length), ints(0, length))
+        outs.append(backend.kv_cache_attention(q, cache, table, ints(length), ints(0, new)))
+    clean, *rest = outs
+    first = max(0, at // 16 * 16 - (length - new))               # row of the page's first token
+    for out in rest:
+        assert torch.equal(out[:first], clean[:first])
+        assert torch.isnan(out[first:]).all()
+    backend.check_status()
