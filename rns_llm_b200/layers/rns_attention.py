@@ -19,7 +19,8 @@ class QuantizedDecoderCache:
 
     Passed to the model as ``past_key_values``; the model asks it for the cached length, the
     attention blocks write to it and read it.  ``max_tokens`` bounds the sequences; a call beyond
-    it raises.  Batches are not padded: every sequence gets the same number of tokens a call.  The
+    it raises.  Batches are not padded: every sequence gets the same number of tokens a call, and
+    each token sees those up to itself; a block refuses any other attention mask.  The
     lengths are counted on the host too, so its calls are not captured into CUDA graphs (the backend's
     own calls can be).
     """
@@ -122,8 +123,8 @@ class QuantizedCacheAttention(nn.Module):
         if self.training:
             raise ValueError("attention over a quantised cache is for inference")
         batch, new, width = hidden_states.shape
-        if self.layer_idx == 0 and new > 1 and attention_mask is not None:
-            _refuse_padding(attention_mask)
+        if attention_mask is not None:
+            _check_mask(attention_mask, batch, block.num_heads, past_key_values.get_seq_length(self.layer_idx), new)
         q, k, v = (proj(hidden_states) for proj in (block.q_proj, block.k_proj, block.v_proj))
         heads = (batch * new, block.num_heads, block.head_dim)
         out = past_key_values.attend(self.layer_idx, q.view(heads), k.view(heads), v.view(heads),
@@ -131,9 +132,23 @@ class QuantizedCacheAttention(nn.Module):
         return block.out_proj(out.view(batch, new, width)), None
 
 
-def _refuse_padding(mask: torch.Tensor) -> None:
-    """The last query of an unpadded batch sees every key."""
-    last = mask[..., -1, :] if mask.ndim == 4 else mask
-    seen = last if last.dtype == torch.bool else (last == 0 if mask.ndim == 4 else last != 0)
-    if not bool(seen.all()):
-        raise ValueError("padded batches are not supported by the quantised cache")
+def _check_mask(mask, batch: int, heads: int, cached: int, new: int) -> None:
+    """Refuses every mask but one that says what the cache's attention does anyway: causal, nothing padded.
+    Reads the mask on the host (the model passes none for unpadded prompts and single tokens, unless its
+    attention is the eager one)."""
+    total = cached + new
+    shape = tuple(mask.shape) if isinstance(mask, torch.Tensor) else ()
+    if len(shape) == 2 and shape[0] in (1, batch) and shape[1] == total:
+        good = mask != 0
+    elif (len(shape) == 4 and shape[0] in (1, batch) and shape[1] in (1, heads) and shape[2:] == (new, total) and
+          (mask.dtype == torch.bool or mask.is_floating_point())):
+        at = torch.arange(total, device=mask.device)
+        seen = at <= at[cached:, None]
+        # scores get 0 added where a key is seen; a type's lowest value or -inf hides it
+        good = mask == seen if mask.dtype == torch.bool else torch.where(seen, mask == 0, mask <= -1e4)
+    else:
+        raise ValueError(f"the quantised cache takes attention masks of [batch, {total}], or boolean or floating ones of "
+                         f"[batch, 1, {new}, {total}]")
+    if not bool(good.all()):
+        raise ValueError("the attention mask is not the causal one: padded batches and masks of other forms are not "
+                         "supported by the quantised cache")
