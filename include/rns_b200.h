@@ -642,7 +642,9 @@ RNS_API int rns_kv_read(const rns_kv_cache* cache, const int32_t* d_first, const
  * 2^-11 of itself, or, where p_j times its page's value scale lies 2^14 or more below the row's
  * largest such product, by 2^-24 of that product at most.
  * max_new: as rns_kv_write.  d_workspace: rns_kv_attention_workspace() bytes of scratch of the
- * caller's stream, 16-byte aligned; nothing in it has to be initialised.
+ * caller's stream, 16-byte aligned; nothing in it has to be initialised.  A call launches two to
+ * four kernels over it: host threads that share a stream do not share a workspace, or make their
+ * calls one after the other.
  */
 typedef struct rns_kv_attention_args {
     const void* d_q;

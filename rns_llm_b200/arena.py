@@ -6,7 +6,9 @@ that never shrinks (``layers/rns_linear.py:206-223``,
 would race.  Here each CUDA stream owns ONE growable byte buffer; every call
 carves its temporaries from the start of it.  Work on a stream executes in
 order, so the next call on the same stream may reuse the same bytes, and two
-streams never share a buffer.
+streams never share a buffer.  A call launches several kernels over its bytes, and
+another host thread may use the same stream (the default one, say): a call holds
+``lock`` from its first use of the buffer to its last launch.
 
 Nothing is allocated while a CUDA graph is being captured: a buffer that would
 have to grow then raises, so warm the shape up once before capturing.
@@ -50,7 +52,7 @@ class StreamArena:
     def __init__(self, initial_bytes: int = 1 << 20) -> None:
         self._initial = int(initial_bytes)
         self._buffers: dict[tuple[int, int], torch.Tensor] = {}
-        self._lock = threading.Lock()
+        self.lock = threading.RLock()
 
     def frame(self, device: torch.device) -> ArenaFrame:
         index = device.index if device.index is not None else torch.cuda.current_device()
@@ -80,7 +82,7 @@ class StreamArena:
                 "shapes once on this stream before capturing"
             )
         size = max(self._initial, 1 << (int(need) - 1).bit_length())
-        with self._lock:
+        with self.lock:
             new = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", key[0]))
             # Earlier slices of the old buffer handed out in this frame stay valid:
             # tensors keep their storage alive, and the caching allocator only

@@ -709,7 +709,7 @@ class CudaRNSBackend(KVCacheOperators):
         self._stats["encode_centered_values"] += int(a.numel())
         self._stats["fused_gemm_calls"] += 1
         self._stats[f"fused_gemm_channels_{channels}"] += 1
-        with torch.cuda.device(a.device):
+        with self.arena.lock, torch.cuda.device(a.device):
             if (_active is None and a.stride(1) == 1 and
                     self._lib.rns_linear_small_supported(m, prepared_weight.k, channels)):
                 # Few tokens (merged single-token requests): one launch, no scratch.
@@ -815,7 +815,7 @@ class CudaRNSBackend(KVCacheOperators):
                 raise ValueError("workspace shape does not match operation")
         out = workspace.output if workspace is not None else torch.empty(
             (m, full.n), dtype=torch.int64, device=device)
-        with torch.cuda.device(device):
+        with self.arena.lock, torch.cuda.device(device):
             frame = self.arena.frame(device)
             scratch = frame.alloc(8, torch.int32)          # [0] row-L1 max, [1] active channels
             meta = torch.empty(3, dtype=torch.int64, device=device) if return_metadata else None
@@ -985,7 +985,7 @@ class CudaRNSBackend(KVCacheOperators):
             # Few tokens on a weight whose K the one-launch kernel cannot hold (and which is not
             # large: from K*N = 2^23 the two-CTA kernel measured faster): quantise to plain int8
             # (one or two small launches), then ONE launch that streams the weight once.
-            with torch.cuda.device(device):
+            with self.arena.lock, torch.cuda.device(device):
                 scale_bytes = ((m if per_row else 1) * 4 + 255) & ~255
                 base, stream = self.arena.block(device, scale_bytes + 256 + m * k)
                 scale, scratch, act = base, base + scale_bytes, base + scale_bytes + 256
@@ -1020,7 +1020,7 @@ class CudaRNSBackend(KVCacheOperators):
         if out_copies and tile_rows == 0:
             raise ValueError("out_copies need the many-token kernel")
         meta = None
-        with torch.cuda.device(device):
+        with self.arena.lock, torch.cuda.device(device):
             # One block of the stream's arena, addressed by offsets (256-byte aligned):
             # scale [M or 1] f32 | scratch 8 x i32 ([0..3] absmax, [4] row-L1 max,
             # [5] active channels) | packed activations (int8, or R planes).
@@ -1106,7 +1106,7 @@ class CudaRNSBackend(KVCacheOperators):
         device = a.device
         out = torch.empty((groups, m_pad, n), dtype=out_dtype, device=device)
         prepared = PreparedRNSWeight(backend=self, moduli=mods, k=k, n=n, kernel="tcgen05")
-        with torch.cuda.device(device):
+        with self.arena.lock, torch.cuda.device(device):
             stream = self._stream(device)
             frame = self.arena.frame(device)
             tile_rows = token_tile // 2
@@ -1162,7 +1162,7 @@ class CudaRNSBackend(KVCacheOperators):
             out = torch.empty((m, prepared.n), dtype=x.dtype, device=device)
         elif out.shape != (m, prepared.n) or out.stride(1) != 1 or out.dtype != x.dtype:
             raise ValueError("out must be [M,N] of x's dtype with unit inner stride")
-        with torch.cuda.device(device):
+        with self.arena.lock, torch.cuda.device(device):
             scale_bytes = ((m if per_row else 1) * 4 + 255) & ~255
             act_bytes = int(self._lib.rns_packed_planes_bytes(m, k, channels, tile_rows))
             base, stream = self.arena.block(device, scale_bytes + 256 + act_bytes)

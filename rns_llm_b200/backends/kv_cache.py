@@ -184,7 +184,7 @@ class KVCacheOperators:
             dim ** -0.5 if softmax_scale is None else softmax_scale, out.data_ptr(), out.stride(0), out.stride(1),
             None if lse is None else lse.data_ptr(), None, 0)
         self._stats["kv_attention_calls"] += 1
-        with _on(device):
+        with self.arena.lock, _on(device):
             need = self._lib.rns_kv_attention_workspace(C.byref(cache_args), C.byref(args))
             if need < 0:
                 N.check(-need)
