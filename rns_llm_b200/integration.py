@@ -58,14 +58,21 @@ def replace_opt_attention_blocks(model: nn.Module, *, backend, blocks: int | Non
 def use_quantized_cache(model: nn.Module) -> list[str]:
     """Wraps every OPT attention module of ``model`` (those with the four projections, replaced by RNS
     linears or not) so that it attends over a ``QuantizedDecoderCache`` passed as ``past_key_values``.
-    Returns their names.  No counterpart in the reference, whose cache stays in floating point."""
-    names = [name for name, module in model.named_modules()
-             if all(isinstance(getattr(module, attr, None), nn.Module) for attr in ("q_proj", "k_proj", "v_proj", "out_proj"))]
+    Returns their names, those wrapped before included; modes (training or not) stay as they are.  No
+    counterpart in the reference, whose cache stays in floating point."""
+    modules = list(model.named_modules())
+    inner = {id(module.attention) for _, module in modules if isinstance(module, QuantizedCacheAttention)}
+    names = []
+    for name, module in modules:
+        if isinstance(module, QuantizedCacheAttention):
+            names.append(name)
+        elif id(module) not in inner and all(isinstance(getattr(module, attr, None), nn.Module)
+                                             for attr in ("q_proj", "k_proj", "v_proj", "out_proj")):
+            parent, attribute = find_parent(model, name)
+            setattr(parent, attribute, QuantizedCacheAttention(module))
+            names.append(name)
     if not names:
         raise ValueError("the model has no attention modules with q_proj, k_proj, v_proj and out_proj")
-    for name in names:
-        parent, attribute = find_parent(model, name)
-        setattr(parent, attribute, QuantizedCacheAttention(getattr(parent, attribute)).eval())
     return names
 
 

@@ -111,6 +111,7 @@ class QuantizedCacheAttention(nn.Module):
             raise ValueError("the attention block has no layer_idx")
         self.attention = attention
         self.layer_idx = int(layer_idx)
+        self.training = attention.training
 
     def forward(self, hidden_states: torch.Tensor, past_key_values=None, attention_mask: torch.Tensor | None = None,
                 output_attentions: bool = False, **kwargs):

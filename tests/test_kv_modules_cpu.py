@@ -175,3 +175,34 @@ def test_model_refuses_padding_and_custom_masks():
             assert cache.get_seq_length() == 6
             model(input_ids=IDS[:, 6:7], past_key_values=cache, use_cache=True)
             assert cache.get_seq_length() == 7
+
+
+def test_wrapping_twice_changes_nothing():
+    model = small_opt()
+    names = use_quantized_cache(model)
+    blocks = [layer.self_attn for layer in model.model.decoder.layers]
+    assert names == [f"model.decoder.layers.{i}.self_attn" for i in range(2)]
+    assert use_quantized_cache(model) == names
+    for layer, block in zip(model.model.decoder.layers, blocks):
+        assert layer.self_attn is block and not isinstance(block.attention, QuantizedCacheAttention)
+    with torch.no_grad():
+        out = model(input_ids=IDS[:, :6], past_key_values=cache_for(model), use_cache=True)
+    assert torch.isfinite(out.logits).all()
+    # a block that was wrapped by hand beside one that was not
+    model = small_opt()
+    layers = model.model.decoder.layers
+    layers[0].self_attn = QuantizedCacheAttention(layers[0].self_attn)
+    first = layers[0].self_attn
+    assert use_quantized_cache(model) == names and layers[0].self_attn is first
+    assert isinstance(layers[1].self_attn, QuantizedCacheAttention)
+
+
+@pytest.mark.parametrize("training", [False, True])
+def test_wrapping_keeps_the_mode_of_a_model(training):
+    model = small_opt().train(training)
+    model.model.decoder.layers[1].self_attn.q_proj.eval()
+    modes = [m.training for m in model.modules()]
+    use_quantized_cache(model)
+    for layer in model.model.decoder.layers:
+        assert layer.self_attn.training == training
+    assert [m.training for m in model.modules() if not isinstance(m, QuantizedCacheAttention)] == modes
