@@ -123,6 +123,8 @@ class QuantizedCacheAttention(nn.Module):
             raise ValueError("attention weights are not formed over a quantised cache")
         if self.training:
             raise ValueError("attention over a quantised cache is for inference")
+        if kwargs.get("key_value_states") is not None:
+            raise ValueError("cross attention does not run on a quantised cache")
         batch, new, width = hidden_states.shape
         if attention_mask is not None:
             _check_mask(attention_mask, batch, block.num_heads, past_key_values.get_seq_length(self.layer_idx), new)

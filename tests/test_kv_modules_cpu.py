@@ -206,3 +206,16 @@ def test_wrapping_keeps_the_mode_of_a_model(training):
     for layer in model.model.decoder.layers:
         assert layer.self_attn.training == training
     assert [m.training for m in model.modules() if not isinstance(m, QuantizedCacheAttention)] == modes
+
+
+def test_keys_of_another_sequence_are_refused():
+    """A block that is given other hidden states for its keys (cross attention) does not run on the cache."""
+    model = small_opt()
+    use_quantized_cache(model)
+    block, x = model.model.decoder.layers[0].self_attn, torch.randn(2, 4, 64).bfloat16()
+    cache = cache_for(model)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="cross"):
+            block(x, past_key_values=cache, key_value_states=x)
+        assert cache.get_seq_length() == 0
+        block(x, past_key_values=cache, key_value_states=None)
