@@ -300,7 +300,7 @@ template <typename T, int FORMAT>
 static int launch_read(const KvView& c, const int32_t* first, const int32_t* row_starts, int64_t rows, int max_rows,
                        void* k, void* v, cudaStream_t st) {
     const int chunk_rows = kReadThreads * kReadVectors * 16 / c.head_dim;
-    const dim3 grid((unsigned)((max_rows + chunk_rows - 1) / chunk_rows), (unsigned)(2 * c.kv_heads), (unsigned)c.sequences);
+    const dim3 grid((unsigned)max(1, (max_rows + chunk_rows - 1) / chunk_rows), (unsigned)(2 * c.kv_heads), (unsigned)c.sequences);
     kv_read_kernel<T, FORMAT><<<grid, kReadThreads, 0, st>>>(c, first, row_starts, rows, max_rows, static_cast<T*>(k),
                                                              static_cast<T*>(v), chunk_rows);
     RNS_CUDA_OK(cudaGetLastError());
@@ -337,7 +337,7 @@ extern "C" int rns_kv_write(const rns_kv_cache* cache, const void* d_k_new, cons
     if (int rc = make_kv_view(cache, &c)) return rc;
     if (tokens < 0 || tokens > INT32_MAX || max_new < 0) return fail(RNS_ERR_INVALID_ARGUMENT, "token counts must be in [0, 2^31)");
     if (type != RNS_F16 && type != RNS_BF16 && type != RNS_F32) return fail(RNS_ERR_INVALID_ARGUMENT, "unknown float type %d", (int)type);
-    if (c.sequences == 0 || tokens == 0 || max_new == 0) return RNS_OK;
+    if (c.sequences == 0 || tokens == 0) return RNS_OK;              // (a bound of zero: what exceeds it is flagged)
     if (!d_k_new || !d_v_new || !d_seq_lens || !d_query_starts) return fail(RNS_ERR_INVALID_ARGUMENT, "a pointer is NULL");
     if (max_new > tokens) max_new = (int)tokens;
     const KvSource src = {{d_k_new, d_v_new}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}};
@@ -363,7 +363,7 @@ extern "C" int rns_kv_read(const rns_kv_cache* cache, const int32_t* d_first, co
     if (int rc = make_kv_view(cache, &c)) return rc;
     if (rows < 0 || rows > INT32_MAX || max_rows < 0) return fail(RNS_ERR_INVALID_ARGUMENT, "row counts must be in [0, 2^31)");
     if (type != RNS_F16 && type != RNS_BF16 && type != RNS_F32) return fail(RNS_ERR_INVALID_ARGUMENT, "unknown float type %d", (int)type);
-    if (c.sequences == 0 || rows == 0 || max_rows == 0) return RNS_OK;
+    if (c.sequences == 0 || rows == 0) return RNS_OK;
     if (!d_first || !d_row_starts || !d_k_out || !d_v_out) return fail(RNS_ERR_INVALID_ARGUMENT, "a pointer is NULL");
     if ((reinterpret_cast<uintptr_t>(d_k_out) | reinterpret_cast<uintptr_t>(d_v_out)) & 15)
         return fail(RNS_ERR_INVALID_ARGUMENT, "outputs must be 16-byte aligned");

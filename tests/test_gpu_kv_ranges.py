@@ -274,3 +274,27 @@ def test_written_infinity_reaches_the_rows_that_see_it(backend, fmt, dim, length
         assert torch.equal(out[:first], clean[:first])
         assert torch.isnan(out[first:]).all()
     backend.check_status()
+
+
+# ---------------------------------------------------------------------------------------
+# bounds of zero
+# ---------------------------------------------------------------------------------------
+def test_a_bound_of_zero_is_reported(backend):
+    """Tokens or rows that a bound of zero leaves out are flagged, as with any bound that is too small."""
+    s = Setup(backend, [40, 20], seed=2)
+    x = torch.ones(2, 2, 64, dtype=torch.float16, device="cuda")
+    lens, starts = s.ints([40, 20]), s.ints([0, 1, 2])
+    backend.kv_cache_write(s.cache, x, x, s.d_table, lens, starts, max_query_len=0)
+    with pytest.raises(RuntimeError, match="out of range"):
+        backend.check_status()
+    s.check_bytes()
+    out = tuple(torch.full((5, 2, 64), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    backend.kv_cache_read(s.cache, s.d_table, s.ints([0, 0]), s.ints([0, 2, 5]), rows=5, max_rows=0, out=out)
+    with pytest.raises(RuntimeError, match="out of range"):
+        backend.check_status()
+    assert (out[0] == 7.0).all() and (out[1] == 7.0).all()
+    # sequences without tokens stay within it
+    backend.kv_cache_write(s.cache, x, x, s.d_table, lens, s.ints([0, 0, 0]), max_query_len=0)
+    backend.kv_cache_read(s.cache, s.d_table, s.ints([0, 0]), s.ints([0, 0, 0]), rows=5, max_rows=0, out=out)
+    backend.check_status()
+    s.check_bytes()
