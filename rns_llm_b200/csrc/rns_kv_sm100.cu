@@ -15,6 +15,8 @@
 // 55 us with the block held as floats); reading 65537 x 8 x 128 to bf16 78 us, 0.79 of it.
 #include "rns_kv.cuh"
 
+#include <algorithm>
+
 namespace rns {
 
 int make_kv_view(const rns_kv_cache* c, KvView* v) {
@@ -141,8 +143,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VECTOR ? 1024 / THR
     const int from = max(s.length - s.count, 0);                  // tokens before position 0 have no place
     if (s.length <= from) return;
     const int nth = (from >> c.page_shift) + blockIdx.x;
+    if (nth > (s.length - 1) >> c.page_shift) return;              // (page numbers: a position there may pass 2^31)
     const int page_from = nth << c.page_shift;
-    if (page_from >= s.length) return;
     const int32_t named = kv_entry(c, b, nth);                     // looked at when the new tokens are on their way
     const int row0 = max(from - page_from, 0), row1 = min(s.length - page_from, c.page_tokens);
     const int groups = c.head_dim >> 3;                            // groups of 8 elements in a row
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && VECTOR ? 1024 / THR
 template <typename T, int FORMAT>
 static int launch_write(const KvView& c, const KvSource& src, const int32_t* lens, const int32_t* starts,
                         int64_t tokens, int max_new, bool vector, cudaStream_t st) {
-    const dim3 grid((unsigned)((max_new + c.page_tokens - 2) / c.page_tokens + 1), (unsigned)(2 * c.kv_heads),
+    const dim3 grid((unsigned)(((int64_t)max_new + c.page_tokens - 2) / c.page_tokens + 1), (unsigned)(2 * c.kv_heads),
                     (unsigned)c.sequences);
     // A CTA holds its block in registers, eight groups of eight elements a thread: the fewest threads that can,
     // so that an SM has many blocks in flight (pages of 32 x 128, bf16 to e4m3: 43 us with 128 threads, 36 with 64).
@@ -300,7 +302,7 @@ template <typename T, int FORMAT>
 static int launch_read(const KvView& c, const int32_t* first, const int32_t* row_starts, int64_t rows, int max_rows,
                        void* k, void* v, cudaStream_t st) {
     const int chunk_rows = kReadThreads * kReadVectors * 16 / c.head_dim;
-    const dim3 grid((unsigned)max(1, (max_rows + chunk_rows - 1) / chunk_rows), (unsigned)(2 * c.kv_heads), (unsigned)c.sequences);
+    const dim3 grid((unsigned)std::max<int64_t>(1, ((int64_t)max_rows + chunk_rows - 1) / chunk_rows), (unsigned)(2 * c.kv_heads), (unsigned)c.sequences);
     kv_read_kernel<T, FORMAT><<<grid, kReadThreads, 0, st>>>(c, first, row_starts, rows, max_rows, static_cast<T*>(k),
                                                              static_cast<T*>(v), chunk_rows);
     RNS_CUDA_OK(cudaGetLastError());

@@ -298,3 +298,37 @@ def test_a_bound_of_zero_is_reported(backend):
     backend.kv_cache_read(s.cache, s.d_table, s.ints([0, 0]), s.ints([0, 0, 0]), rows=5, max_rows=0, out=out)
     backend.check_status()
     s.check_bytes()
+
+
+# ---------------------------------------------------------------------------------------
+# positions near 2^31
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,window", [(1, 200), (5, 3000), (300, 200)])
+def test_positions_near_the_end_of_32_bits(backend, new, window):
+    """The longest sequence that a page table may describe (its pages but the last few shared), beside one whose
+    many new tokens make the grid of a write reach beyond 2^31 from there."""
+    page, width = 128, 2 ** 24 - 33
+    length, other = width * page, 9000
+    own = 40                                                     # last pages of the long sequence
+    cache, small = (backend.create_kv_cache(pages=1 + own + 71, kv_heads=1, head_dim=16, page_tokens=page) for _ in range(2))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    tail = torch.arange(1, 1 + own, dtype=torch.int32, device="cuda")
+    beside = torch.arange(1 + own, 1 + own + 71, dtype=torch.int32, device="cuda")
+    table = torch.zeros((2, width), dtype=torch.int32, device="cuda")
+    table[0, -own:], table[1, :71] = tail, beside
+    small_table = torch.zeros((2, 71), dtype=torch.int32, device="cuda")
+    small_table[0, :own], small_table[1] = tail, beside
+    gen = torch.Generator(device="cuda").manual_seed(new)
+    k, v = (torch.randn(new + other, 1, 16, generator=gen, device="cuda").half() for _ in range(2))
+    before = [torch.randn(own * page - new, 1, 16, generator=gen, device="cuda").half() for _ in range(2)]
+    q = torch.randn(new, 2, 16, generator=gen, device="cuda").half()
+    results = []
+    for c, t, n in ((cache, table, length), (small, small_table, own * page)):
+        backend.kv_cache_write(c, *before, small_table[:1], ints(own * page - new), ints(0, own * page - new))
+        backend.kv_cache_write(c, k, v, t, ints(n, other), ints(0, new, new + other))
+        read = backend.kv_cache_read(c, t, ints(n - 700, 5), ints(0, 700, other + 695), rows=other + 695)
+        out = backend.kv_cache_attention(q, c, t[:1], ints(n), ints(0, new), window=window, return_lse=True)
+        results.append((c.k, c.v, c.k_scale, c.v_scale, *read, *out))
+    backend.check_status()
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
