@@ -301,9 +301,16 @@ __device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity, volat
     return ok;
 }
 
+// What a warp still has on its way lands before it leaves, also when a wait has expired: a wait of its own limit.
+__device__ __forceinline__ void prompt_drain(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < 10000 && !prompt_poll(bar, parity); ++i) {}
+}
+
 struct PromptBars {
     uint64_t raw_full[4], raw_empty[4], full[4], empty[4], s_full[2], p_ready[2], o_full[2], q_full[2];
     uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots], part_full[kPartSlots], part_empty[kPartSlots];
+    uint64_t drained;                     // products that were on their way when a wait expired
 };
 struct PromptScales {
     float key[8], exponent[8], weight[8], back[8];   // of 16 keys each: key scale, and the value scale's kv_value_scale
@@ -446,6 +453,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             mbar_init(smem_addr(&bars.part_full[i]), 1);
             mbar_init(smem_addr(&bars.part_empty[i]), 15);         // every warp but the one that writes them
         }
+        mbar_init(smem_addr(&bars.drained), 1);
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -874,6 +882,11 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             // nothing may still be on its way to this CTA's barriers when it leaves
             for (uint32_t i = n > S::kRing ? n - S::kRing : 0; i < n && ok; ++i)
                 wait(bars.empty[i % S::kRing], i / S::kRing, 10, i % S::kRing);
+            if (!ok) {                                             // nor read and write memory that is given back
+                if (elect_one()) umma_commit(smem_addr(&bars.drained));
+                __syncwarp();
+                prompt_drain(smem_addr(&bars.drained), 0);
+            }
         } else if (warp == kCopyWarp) {
             // ------------------------------------------------------------------ copies
             uint32_t n = 0;
@@ -918,6 +931,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 }
                 part_done();
             }
+            for (uint32_t i = n > S::kRawRing ? n - S::kRawRing : 0; i < n; ++i)
+                prompt_drain(smem_addr(&bars.raw_full[i % S::kRawRing]), (i / S::kRawRing) & 1);
         } else if (warp == kScaleWarp) {
             // ------------------------------------------------------------------ scales of the pages
             uint32_t n = 0;
