@@ -7,6 +7,7 @@ GPU is needed to build.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -29,6 +30,31 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC,-fvisibility=hidden",
     "--expt-relaxed-constexpr",
 ]
+
+# Kernels that split their registers anew among their warps count on this many a thread at launch: a split of
+# more than the block was launched with would wait for ever.  The compiler may use fewer, so the build looks.
+LEAST_REGISTERS = {"rns_kv_prompt_sm100.cu": ("kv_prompt_kernel", 128)}
+
+
+def check_registers(source: str, report: str) -> None:
+    """Raises if ``report``, the assembler's resource usage of ``source`` (-Xptxas -v), shows a kernel of
+    LEAST_REGISTERS with fewer registers than it needs, or none of its instances."""
+    if source not in LEAST_REGISTERS:
+        return
+    kernel, least = LEAST_REGISTERS[source]
+    used, entry = {}, None
+    for line in report.splitlines():
+        found = re.search(r"Compiling entry function '(\w+)'", line)
+        if found:
+            entry = found.group(1)
+        found = re.search(r"Used (\d+) registers", line)
+        if found and entry is not None and kernel in entry:
+            used[entry] = int(found.group(1))
+    if not used:
+        raise RuntimeError(f"the assembler's report of {source} names no {kernel}")
+    for entry, registers in used.items():
+        if registers < least:
+            raise RuntimeError(f"{source}: {entry} was compiled to {registers} registers, its split needs {least}")
 
 
 def _nvcc() -> str:
@@ -56,14 +82,15 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     nvcc = _nvcc()
     objdir = HERE / "build"
     objdir.mkdir(exist_ok=True)
-    extra = ["-Xptxas", "-v"] if verbose else []
 
     def compile_one(src: Path) -> Path:
         obj = objdir / (src.stem + ".o")
+        extra = ["-Xptxas", "-v"] if verbose or src.name in LEAST_REGISTERS else []
         cmd = [nvcc, *NVCC_FLAGS, *extra, "-c", str(src), "-o", str(obj)]
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"nvcc failed for {src.name}:\n{proc.stdout}\n{proc.stderr}")
+        check_registers(src.name, proc.stderr)
         if verbose:
             sys.stderr.write(proc.stderr)
         return obj

@@ -50,7 +50,8 @@ constexpr int kScaleSlots = 4, kPartSlots = 4;
 // without, 39.0 / 38.4 / 37.1).
 constexpr int kItemCost = 3;
 // Registers: a softmax thread holds its row's scores of a block.  8 warps of kSoftmaxRegs and 8 of kOtherRegs
-// must not exceed what the block was launched with, 16 warps of kLaunchRegs.
+// must not exceed what the block was launched with, 16 warps of kLaunchRegs (build.py refuses to build the kernel
+// with fewer).
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(8 * kSoftmaxRegs + 8 * kOtherRegs <= 16 * kLaunchRegs, "register split");
 
@@ -1086,7 +1087,7 @@ template <int DIM, int FORMAT> static int launch_prompt(PromptParams& p, void* w
     p.meta = static_cast<int32_t*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (int64_t)sms * 32);
     const auto kernel = kv_prompt_kernel<DIM, FORMAT>;
-    // the kernel's own split of the registers counts on this launch (looked up once per process)
+    // a library that was built some other way: the split of the registers counts on this launch (looked up once)
     static const int regs = [&] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0; }();
     if (regs < kLaunchRegs) return fail(RNS_ERR_UNSUPPORTED, "the prompt kernel was built with %d registers, not %d", regs, kLaunchRegs);
     static std::atomic<uint64_t> allowed{0};
