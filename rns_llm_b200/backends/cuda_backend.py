@@ -250,6 +250,10 @@ class CudaRNSBackend(KVCacheOperators):
         index = device.index if device.index is not None else torch.cuda.current_device()
         state = self._device_state.get(index)
         if state is None:
+            if torch.cuda.is_current_stream_capturing():
+                # the graph would own the words and clear them in every replay
+                raise RuntimeError("the first call of a backend on a device cannot be captured into a CUDA graph; run "
+                                   "one before capturing")
             dev = torch.device("cuda", index)
             state = _DeviceState(
                 status=torch.zeros(1, dtype=torch.int32, device=dev),

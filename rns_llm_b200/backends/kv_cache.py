@@ -82,7 +82,9 @@ class KVCacheOperators:
         shape = (int(pages), int(kv_heads), int(page_tokens), int(head_dim))
         k, v = (torch.zeros(shape, dtype=torch.int8, device=device).view(_FORMAT_NAMES[format]) for _ in range(2))
         k_scale, v_scale = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
-        return QuantizedKVCache(k=k, v=v, k_scale=k_scale, v_scale=v_scale)
+        cache = QuantizedKVCache(k=k, v=v, k_scale=k_scale, v_scale=v_scale)
+        self._state(cache.device)                    # calls on it may be captured from the first on
+        return cache
 
     def kv_cache_write(self, cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
                        seq_lens: torch.Tensor, query_starts: torch.Tensor, *, max_query_len: int | None = None) -> None:
