@@ -56,6 +56,8 @@ class QuantizedKVCache:
         for scale in (self.k_scale, self.v_scale):
             if scale.shape != k.shape[:2] or scale.dtype != torch.float32 or not scale.is_contiguous():
                 raise ValueError("k_scale and v_scale must be contiguous float32 [pages, kv_heads]")
+        if _spans_meet(k, v) or _spans_meet(self.k_scale, self.v_scale):
+            raise ValueError("k and v, and their scales, must not overlap")
         if not k.is_cuda or any(t.device != k.device for t in (v, self.k_scale, self.v_scale)):
             raise ValueError("the cache must be CUDA tensors on one device")
         pages, heads, page_tokens, dim = (int(x) for x in k.shape)
@@ -134,9 +136,11 @@ class KVCacheOperators:
             out = (torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
         else:
             dtype = out[0].dtype
-            if dtype not in _FLOAT_TYPES or any(
+            if len(out) != 2 or dtype not in _FLOAT_TYPES or any(
                     o.shape != shape or o.dtype != dtype or not o.is_contiguous() or o.device != device for o in out):
                 raise ValueError("out must be two contiguous [rows, kv_heads, head_dim] floating tensors")
+            if _spans_meet(*out):
+                raise ValueError("the two outputs must not overlap")
         args = self._kv_args(cache, page_table, first, row_starts)
         self._stats["kv_read_calls"] += 1
         with _on(device):
@@ -156,7 +160,8 @@ class KVCacheOperators:
         rows ``query_starts[b]:query_starts[b+1]`` and sit at the last positions of its
         ``seq_lens[b]`` tokens; each sees the tokens up to its own (all of them with
         ``causal=False``), and with ``window`` only the last ``window`` of those.  One that sees
-        nothing gets zeros.  Rows of no sequence are not written.  Returns the output in q's type
+        nothing gets zeros.  Rows of no sequence are not written.  ``out``, where given, shares no
+        element with ``q``.  Returns the output in q's type
         and, with ``return_lse``, also float32 [tokens, heads]: the log of the sum of the
         exponentials of the scaled scores (-inf where nothing is seen)."""
         if q.ndim != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.kv_heads or q.shape[1] == 0:
@@ -176,7 +181,7 @@ class KVCacheOperators:
         elif (out.shape != q.shape or out.dtype != q.dtype or out.device != device or
               not (out.is_contiguous() or _rows_apart(out))):
             raise ValueError("out must be [tokens, heads, head_dim] of q's type with separate rows and unit inner stride")
-        elif out.data_ptr() == q.data_ptr() and tokens:
+        elif _rows_meet(out, q):
             raise ValueError("out must not overlap q")
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
         cache_args = self._kv_args(cache, page_table, seq_lens, query_starts)
@@ -265,3 +270,31 @@ def _rows_apart(t: torch.Tensor) -> bool:
                 return False
             need = stride * size
     return True
+
+
+def _spans_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the stretches of memory from the first to the last element of two tensors meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    first, end = zip(*((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
+        stride * (size - 1) for stride, size in zip(t.stride(), t.shape)))) for t in (a, b)))
+    return first[0] < end[1] and first[1] < end[0]
+
+
+def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [a, b, d] tensors of one shape and type, with unit inner stride, share an element.  Exact where
+    their strides are equal (column blocks of one buffer); others are told apart by their spans only."""
+    if not _spans_meet(a, b):
+        return False
+    rows, heads, dim = a.shape
+    apart, odd = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    row, head = (0 if size == 1 else stride for size, stride in zip(a.shape[:2], a.stride()[:2]))
+    if odd or (row, head) != tuple(0 if size == 1 else stride for size, stride in zip(b.shape[:2], b.stride()[:2])):
+        return True
+    # apart = i * row + j * head + k with |i| < rows, |j| < heads, |k| < dim
+    for j in range(1 - heads, heads):
+        rest = apart - j * head
+        for i in ((rest // row, rest // row + 1) if row else (0,)):
+            if abs(i) < rows and abs(rest - i * row) < dim:
+                return True
+    return False

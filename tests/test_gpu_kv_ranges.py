@@ -332,3 +332,24 @@ def test_positions_near_the_end_of_32_bits(backend, new, window):
     backend.check_status()
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------------------
+# outputs that overlap
+# ---------------------------------------------------------------------------------------
+def test_outputs_that_overlap_are_refused(backend):
+    s = Setup(backend, [40, 20])
+    lens, starts = s.ints([40, 20]), s.ints([0, 1, 2])
+    wide = torch.ones(3, 8, 64, dtype=torch.float16, device="cuda")
+    q = wide[:2, :4]
+    for out in (wide[1:, :4], wide[:2, 2:6], wide[:2, :4], wide.view(-1)[64:64 + 512].view(2, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            backend.kv_cache_attention(q, s.cache, s.d_table, lens, starts, out=out)
+    want = backend.kv_cache_attention(q, s.cache, s.d_table, lens, starts)
+    got = backend.kv_cache_attention(q, s.cache, s.d_table, lens, starts, out=wide[:2, 4:])     # beside it
+    assert torch.equal(got, want) and (wide[:, :4] == 1).all() and (wide[2] == 1).all()
+    rows = torch.zeros(5, 2, 64, dtype=torch.float16, device="cuda")
+    for out in ((rows[:3], rows[:3]), (rows[:3], rows[2:]), (rows[:3],), (rows[:3],) * 3):
+        with pytest.raises(ValueError):
+            backend.kv_cache_read(s.cache, s.d_table, s.ints([0, 0]), s.ints([0, 2, 3]), rows=3, out=out)
+    backend.check_status()
