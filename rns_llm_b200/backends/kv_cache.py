@@ -72,6 +72,15 @@ class QuantizedKVCache:
                                    kv_heads=heads, head_dim=dim, format=_FORMATS[k.dtype])
         self.device, self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.device, pages, heads, page_tokens, dim
 
+    # Copies and pickles hold the tensors (as bytes: pickles of 8-bit floats do not load); the addresses are the
+    # new ones'.
+    def __getstate__(self) -> dict:
+        return {"k": self.k.view(torch.int8), "v": self.v.view(torch.int8), "k_scale": self.k_scale,
+                "v_scale": self.v_scale, "type": self.k.dtype}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__init__(state["k"].view(state["type"]), state["v"].view(state["type"]), state["k_scale"], state["v_scale"])
+
 
 class KVCacheOperators:
     """Mixed into ``CudaRNSBackend``."""

@@ -8,6 +8,8 @@ block goes to the module it wraps.
 """
 from __future__ import annotations
 
+import copy
+
 import torch
 from torch import nn
 
@@ -68,6 +70,15 @@ class QuantizedDecoderCache:
         """Forgets the sequences; their pages are taken over by the next ones."""
         self.seq_lens.zero_()
         self._lengths = [0] * len(self.caches)
+
+    def __deepcopy__(self, memo: dict) -> "QuantizedDecoderCache":
+        """A cache of its own with the same sequences, on the same backend."""
+        own = copy.copy(self)
+        memo[id(self)] = own
+        own.caches = copy.deepcopy(self.caches, memo)
+        own.page_table, own.seq_lens = self.page_table.clone(), self.seq_lens.clone()
+        own._lengths, own._starts = list(self._lengths), dict(self._starts)
+        return own
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                softmax_scale: float) -> torch.Tensor:

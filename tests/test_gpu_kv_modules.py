@@ -116,3 +116,40 @@ def test_refusals(backend):
         use_quantized_cache(small)
         with torch.no_grad():
             small(input_ids=ids, past_key_values=QuantizedDecoderCache.for_model(small, backend, batch=2, max_tokens=40))
+
+
+def test_copies_and_pickles(backend):
+    """A copied or unpickled cache has tensors and addresses of its own; a copied conversation goes its own way."""
+    import copy
+    import pickle
+
+    from rns_llm_b200.integration import use_quantized_cache
+    from rns_llm_b200.layers import QuantizedDecoderCache
+
+    for format in ("int8", "e4m3"):
+        cache = backend.create_kv_cache(pages=3, kv_heads=2, head_dim=64, page_tokens=16, format=format)
+        x = torch.randn(20, 2, 64, device="cuda").half()
+        table = torch.tensor([[2, 0]], dtype=torch.int32, device="cuda")
+        ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        backend.kv_cache_write(cache, x, x, table, ints(20), ints(0, 20))
+        want = backend.kv_cache_read(cache, table, ints(0), ints(0, 20), rows=20)
+        for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+            assert other.k.data_ptr() != cache.k.data_ptr() and other.k.dtype == cache.k.dtype
+            for a, b in zip(backend.kv_cache_read(other, table, ints(0), ints(0, 20), rows=20), want):
+                assert torch.equal(a, b)
+            backend.kv_cache_write(other, x * 9, x * 9, table, ints(20), ints(0, 20))
+            for a, b in zip(backend.kv_cache_read(cache, table, ints(0), ints(0, 20), rows=20), want):
+                assert torch.equal(a, b)
+    model = small_opt()
+    use_quantized_cache(model)
+    ids = torch.randint(0, 512, (2, 30), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    with torch.no_grad():
+        first = QuantizedDecoderCache.for_model(model, backend, batch=2, max_tokens=40, page_tokens=16)
+        model(input_ids=ids[:, :20], past_key_values=first, use_cache=True)
+        second = copy.deepcopy(first)
+        model(input_ids=ids[:, 25:], past_key_values=second, use_cache=True)
+        a = model(input_ids=ids[:, 20:25], past_key_values=first, use_cache=True).logits
+        third = QuantizedDecoderCache.for_model(model, backend, batch=2, max_tokens=40, page_tokens=16)
+        model(input_ids=ids[:, :20], past_key_values=third, use_cache=True)
+        assert torch.equal(a, model(input_ids=ids[:, 20:25], past_key_values=third, use_cache=True).logits)
+    backend.check_status()

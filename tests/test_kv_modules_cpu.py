@@ -22,7 +22,8 @@ class PlainBackend:
             raise ValueError("format")
         shape = (pages * page_tokens, kv_heads, head_dim)
         return types.SimpleNamespace(device=torch.device("cpu"), page=page_tokens, kv_heads=kv_heads, head_dim=head_dim,
-                                     k=torch.zeros(shape), v=torch.zeros(shape))
+                                     k=torch.zeros(shape), v=torch.zeros(shape), k_scale=torch.zeros(pages, kv_heads),
+                                     v_scale=torch.zeros(pages, kv_heads))
 
     def rows(self, cache, table, b, n):
         at = torch.arange(n)
@@ -219,3 +220,22 @@ def test_keys_of_another_sequence_are_refused():
             block(x, past_key_values=cache, key_value_states=x)
         assert cache.get_seq_length() == 0
         block(x, past_key_values=cache, key_value_states=None)
+
+
+def test_a_copy_goes_its_own_way():
+    import copy
+
+    model = small_opt()
+    use_quantized_cache(model)
+    cache = cache_for(model)
+    step = lambda c, at, n: model(input_ids=IDS[:, at:at + n], past_key_values=c, use_cache=True).logits
+    with torch.no_grad():
+        step(cache, 0, 6)
+        other = copy.deepcopy(cache)
+        assert other.backend is cache.backend and other.caches[0].k.data_ptr() != cache.caches[0].k.data_ptr()
+        step(other, 9, 3)
+        assert (cache.get_seq_length(), other.get_seq_length()) == (6, 9)
+        assert cache.seq_lens.tolist() == [6, 6] and other.seq_lens.tolist() == [9, 9]
+        fresh = cache_for(model)
+        step(fresh, 0, 6)
+        assert torch.equal(step(cache, 6, 2), step(fresh, 6, 2))
