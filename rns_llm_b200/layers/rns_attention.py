@@ -71,6 +71,15 @@ class QuantizedDecoderCache:
         self.seq_lens.zero_()
         self._lengths = [0] * len(self.caches)
 
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Sequence i becomes a copy of sequence ``beam_idx[i]`` (beam search)."""
+        if tuple(beam_idx.shape) != (self.batch,):
+            raise ValueError(f"beam_idx must name a sequence for each of the cache's {self.batch}")
+        for cache in self.caches:
+            for tensor in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+                rows = tensor.view(torch.int8).view(self.batch, -1)      # a sequence's pages lie together
+                rows.copy_(rows.index_select(0, beam_idx.to(rows.device)))
+
     def __deepcopy__(self, memo: dict) -> "QuantizedDecoderCache":
         """A cache of its own with the same sequences, on the same backend."""
         own = copy.copy(self)

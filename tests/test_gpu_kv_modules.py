@@ -152,4 +152,11 @@ def test_copies_and_pickles(backend):
         third = QuantizedDecoderCache.for_model(model, backend, batch=2, max_tokens=40, page_tokens=16)
         model(input_ids=ids[:, :20], past_key_values=third, use_cache=True)
         assert torch.equal(a, model(input_ids=ids[:, 20:25], past_key_values=third, use_cache=True).logits)
+        # beams: both sequences go on from the second
+        first.reorder_cache(torch.tensor([1, 1], device="cuda"))
+        third.reset()
+        model(input_ids=ids[[1, 1], :20], past_key_values=third, use_cache=True)
+        model(input_ids=ids[[1, 1], 20:25], past_key_values=third, use_cache=True)
+        b, c = (model(input_ids=ids[:, 25:26], past_key_values=x, use_cache=True).logits for x in (first, third))
+        assert torch.equal(b, c)
     backend.check_status()

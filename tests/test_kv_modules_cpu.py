@@ -239,3 +239,40 @@ def test_a_copy_goes_its_own_way():
         fresh = cache_for(model)
         step(fresh, 0, 6)
         assert torch.equal(step(cache, 6, 2), step(fresh, 6, 2))
+
+
+def test_sequences_are_reordered():
+    model = small_opt()
+    use_quantized_cache(model)
+    cache, swapped = cache_for(model), cache_for(model)
+    with torch.no_grad():
+        model(input_ids=IDS[:, :6], past_key_values=cache, use_cache=True)
+        model(input_ids=IDS[[1, 1], :6], past_key_values=swapped, use_cache=True)
+        cache.reorder_cache(torch.tensor([1, 1]))
+        a, b = (model(input_ids=IDS[:, 6:8], past_key_values=c, use_cache=True).logits for c in (cache, swapped))
+    assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="beam_idx"):
+        cache.reorder_cache(torch.tensor([0]))
+
+
+@pytest.mark.parametrize("beams", [1, 3])
+def test_generate(beams):
+    """The model library's search over the cache: greedy tokens are those of single steps by hand, beams follow
+    the sequences that the search keeps."""
+    model = small_opt()
+    use_quantized_cache(model)
+    cache, calls = cache_for(model, batch=2 * beams), []
+    reorder, cache.reorder_cache = cache.reorder_cache, lambda index: calls.append(index) or reorder(index)
+    got = model.generate(IDS[:, :6], attention_mask=torch.ones(2, 6, dtype=torch.long), past_key_values=cache,
+                         max_new_tokens=8, num_beams=beams, do_sample=False, pad_token_id=1, eos_token_id=None)
+    assert got.shape == (2, 14) and torch.equal(got[:, :6], IDS[:, :6])
+    assert cache.get_seq_length() == 13
+    if beams > 1:
+        assert calls and all(tuple(index.shape) == (2 * beams,) for index in calls)
+        return
+    own, tokens, want = cache_for(model), IDS[:, :6], [IDS[:, :6]]
+    with torch.no_grad():
+        for _ in range(8):
+            tokens = model(input_ids=tokens, past_key_values=own, use_cache=True).logits[:, -1:].float().argmax(-1)
+            want.append(tokens)
+    assert torch.equal(got, torch.cat(want, 1))
