@@ -104,17 +104,23 @@ class QuantizedDecoderCache:
         ahead = max(self._lengths)
         if ahead > self._lengths[layer] and ahead != length:
             raise ValueError("the layers of the cache are at different lengths")
-        if ahead < length:                               # the first layer of this call
-            self.seq_lens += new
-        self._lengths[layer] = length
         starts = self._starts.get(new)
         if starts is None:
             starts = torch.arange(0, (self.batch + 1) * new, new, dtype=torch.int32, device=self.seq_lens.device)
             self._starts[new] = starts
         cache = self.caches[layer]
-        self.backend.kv_cache_write(cache, k, v, self.page_table, self.seq_lens, starts, max_query_len=new)
-        return self.backend.kv_cache_attention(q, cache, self.page_table, self.seq_lens, starts, max_query_len=new,
-                                               softmax_scale=softmax_scale)
+        if ahead < length:                               # the first layer of this call
+            self.seq_lens += new
+        try:
+            self.backend.kv_cache_write(cache, k, v, self.page_table, self.seq_lens, starts, max_query_len=new)
+            out = self.backend.kv_cache_attention(q, cache, self.page_table, self.seq_lens, starts, max_query_len=new,
+                                                  softmax_scale=softmax_scale)
+        except Exception:
+            if ahead < length:
+                self.seq_lens -= new
+            raise
+        self._lengths[layer] = length
+        return out
 
 
 class QuantizedCacheAttention(nn.Module):

@@ -276,3 +276,25 @@ def test_generate(beams):
             tokens = model(input_ids=tokens, past_key_values=own, use_cache=True).logits[:, -1:].float().argmax(-1)
             want.append(tokens)
     assert torch.equal(got, torch.cat(want, 1))
+
+
+@pytest.mark.parametrize("where", ["kv_cache_write", "kv_cache_attention"])
+def test_a_call_that_raises_appends_nothing(where, monkeypatch):
+    """The lengths are those before it, and the conversation goes on as if it had not been."""
+    model = small_opt()
+    use_quantized_cache(model)
+    cache, twin = cache_for(model), cache_for(model)
+    step = lambda c, at, n: model(input_ids=IDS[:, at:at + n], past_key_values=c, use_cache=True).logits
+
+    def broken(*args, **kw):
+        raise RuntimeError("out of memory")
+
+    with torch.no_grad():
+        for c in (cache, twin):
+            step(c, 0, 6)
+        with monkeypatch.context() as patch:
+            patch.setattr(cache.backend, where, broken)
+            with pytest.raises(RuntimeError, match="out of memory"):
+                step(cache, 6, 3)
+        assert cache.get_seq_length() == 6 and cache.seq_lens.tolist() == [6, 6]
+        assert torch.equal(step(cache, 6, 2), step(twin, 6, 2))
