@@ -638,9 +638,10 @@ RNS_API int rns_kv_read(const rns_kv_cache* cache, const int32_t* d_first, const
  *   d_out  [tokens, heads, head_dim] of q's type, likewise; rows of no sequence stay as they are
  *   d_lse  float [tokens, heads] or NULL: log of the sum of exp of the scaled scores (-inf where
  *          a query sees nothing)
- * Scores, softmax and sums are fp32.  A softmax weight p_j meets the values rounded to fp16: off by
- * 2^-11 of itself, or, where p_j times its page's value scale lies 2^14 or more below the row's
- * largest such product, by 2^-24 of that product at most.
+ * Scores, softmax and sums are fp32.  A softmax weight p_j meets the values off by 2^-22 of itself
+ * (2^-11 in calls with a sequence of more than 32 query rows, new tokens x heads that share one of
+ * the cache's), or by 2^-24 of the row's largest product of a weight and its page's value scale, if
+ * that is more.
  * max_new: as rns_kv_write.  d_workspace: rns_kv_attention_workspace() bytes of scratch of the
  * caller's stream, 16-byte aligned; nothing in it has to be initialised.  A call launches two to
  * four kernels over it: host threads that share a stream do not share a workspace, or make their

@@ -20,17 +20,20 @@
 //   index costs least: sums do not depend on it, and Q is laid out to match.
 // * Queries are scaled by a power of two per row into fp16's range, exact for bf16 as well up to
 //   2^-32 of the row's largest element.  Scores, the softmax and all sums are fp32.  Each weight, with
-//   its page's value scale, is rounded to fp16 (2^-11) for the second product, in units of a power of
-//   two near the row's largest such weight (kv_value_scale); the accumulators need no scale of their
-//   own.  Weights 2^14 below that are off by up to 2^-25 of the unit each.
+//   its page's value scale, meets the values as two fp16 numbers, itself rounded and what that left
+//   (2^-22), in units of a power of two near the row's largest such weight (kv_value_scale); the
+//   accumulators need no scale of their own.  Small weights are off by up to 2^-25 of the unit each.
+//   Rounded once, outputs in fp16 were off by 0.0003 where rounding the exact result gives 0.0002; the
+//   second part costs 2 to 4 % (64 sequences 142.5 -> 145.5 us, one of 131072 tokens 65.8 -> 68.6; a
+//   branch that leaves it out for bf16, whose own rounding hides it, costs as much: 145.0, 68.1).
 // * The running maximum may lag by 2^8: then weights exceed one but nothing is lost, and the
 //   accumulators are rescaled only when a vote finds a larger score.  It is a whole number, so that
 //   rescaling is exact, and follows the row's own scores and their pages' scales alone: what a row
 //   gives does not depend on the rows beside it.
 //
-// Measured (graph replay): 64 sequences of 1..8192 tokens, 32 over 8 heads of 128, 143 us = 3.75 TB/s of cache
-// (0.58 of the copy rate; 450 instructions for 16 keys, issue slots 53 % busy with three warps a scheduler: the
-// latency of dependent instructions bounds it); one sequence of 131072, e4m3, 68 us; 8 of 640, 12 heads of 64, 16 us.
+// Measured (graph replay): 64 sequences of 1..8192 tokens, 32 over 8 heads of 128, 145 us = 3.70 TB/s of cache
+// (0.57 of the copy rate; about 470 instructions for 16 keys, issue slots 53 % busy with three warps a scheduler: the
+// latency of dependent instructions bounds it); one sequence of 131072, e4m3, 69 us; 8 of 640, 12 heads of 64, 16 us.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 
@@ -500,7 +503,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                     for (int i = 0; i < MT; ++i) { o[i][nt][e] *= keep; o[i][nt][e + 2] *= keep; }
                                 }
                         }
-                        uint32_t pf[NT][2];
+                        uint32_t pf[NT][2], pl[NT][2];                             // weights, and what rounding left of them
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float w[4];
@@ -514,6 +517,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                             const __half2 top = __floats2half2_rn(w[0], w[1]), low = __floats2half2_rn(w[2], w[3]);
                             pf[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&top));
                             pf[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&low));
+                            const float2 t2 = __half22float2(top), l2 = __half22float2(low);
+                            const __half2 top_left = __floats2half2_rn(w[0] - t2.x, w[1] - t2.y);
+                            const __half2 low_left = __floats2half2_rn(w[2] - l2.x, w[3] - l2.y);
+                            pl[nt][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&top_left));
+                            pl[nt][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&low_left));
                         }
                         // values: keys 2c, 2c+1, 2c+8, 2c+9; 16 (DIM 64: 8) dimensions of this thread
                         const bool tail = FORMAT == RNS_KV_E4M3 && k0 + 16 > it.length;
@@ -547,6 +555,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt)
                                         mma_f16(o[part * 8 + w * 2 + h][nt], a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1], pf[nt][0], pf[nt][1]);
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt)
+                                        mma_f16(o[part * 8 + w * 2 + h][nt], a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1], pl[nt][0], pl[nt][1]);
                             }
                         }
                     }

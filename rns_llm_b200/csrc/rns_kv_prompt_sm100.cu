@@ -19,7 +19,9 @@
 // * Numerics are those of the rows kernel: queries times a power of two per row, fp32 scores, softmax
 //   and sums, weights with their pages' value scales rounded to fp16 in units of a power of two near the
 //   row's largest; the running maximum may lag by 2^8, so that O in tensor memory is rescaled only now
-//   and then.
+//   and then.  Weights are rounded once: outputs in fp16 are off by 0.0003 where rounding the exact result
+//   gives 0.0002.  A second part of each weight, as the rows kernel has, brings 0.0002 and costs a second
+//   product on the chain: a prompt of 4096 tokens 266 us for 235, the chunk 390 for 333.
 // * Work is cut as there: one axis of key blocks over all items, equal shares, pieces joined by a
 //   second kernel.
 //

@@ -211,6 +211,27 @@ def test_pages_of_zeros(backend, new):
     assert (got[new:] == 0).all()
 
 
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("dim,fmt,heads", [(64, "int8", 4), (128, "int8", 8), (80, "e4m3", 4), (256, "e4m3", 2)])
+def test_few_rows_are_as_exact_as_their_type(backend, dim, fmt, heads, new):
+    """Weights meet the values in two fp16 parts, so an fp16 output is off by its own rounding and little else: the
+    error's norm is within a tenth of that of the exact result rounded (weights rounded once make it 1.4 times)."""
+    lens = [600] * 8
+    s = Setup(backend, lens, kv_heads=2, dim=dim, page=64, fmt=fmt, seed=dim, spread=0.1)
+    for scale in s.scale[0]:
+        scale[:] = 2 / (float(O.LARGEST[fmt]) / 3)               # scores with a spread of 2
+    s.to_device()
+    q = queries(s, 8 * new, heads, dim)
+    got, _ = attend(backend, s, q, [new] * 8)
+    wrong = rounded = 0.0
+    for b in range(8):
+        rows = slice(b * new, (b + 1) * new)
+        want = O.attention(q[rows].float().numpy(), s.values(b, 0), s.values(b, 1), 600, scale=dim ** -0.5)[0]
+        wrong += float(((got[rows].double().cpu().numpy() - want) ** 2).sum())
+        rounded += float(((want.astype(np.float16).astype(np.float64) - want) ** 2).sum())
+    assert wrong <= 1.1 ** 2 * rounded, (wrong / rounded) ** 0.5
+
+
 # ---------------------------------------------------------------------------------------
 # values that are not finite
 # ---------------------------------------------------------------------------------------
