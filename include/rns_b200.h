@@ -572,7 +572,7 @@ typedef enum rns_kv_format {
  * *d_status = RNS_ERR_BAD_INDEX and touches no memory: a sequence with a bad length or start
  * counts as empty, a bad page is not written and reads as zeros.
  * Sequences may share pages that are only read; a page that is written must belong to one
- * sequence of the call.
+ * sequence of the call and stand once in its row of the table.
  */
 typedef struct rns_kv_cache {
     int8_t* d_k;
@@ -642,7 +642,8 @@ RNS_API int rns_kv_read(const rns_kv_cache* cache, const int32_t* d_first, const
  * (2^-11 in calls with a sequence of more than 32 query rows, new tokens x heads that share one of
  * the cache's), or by 2^-24 of the row's largest product of a weight and its page's value scale, if
  * that is more.
- * max_new: as rns_kv_write.  d_workspace: rns_kv_attention_workspace() bytes of scratch of the
+ * max_new: no sequence of the call has more new tokens.  It only chooses kernels and tiles here: one
+ * that is too small or far too large costs time, not results.  d_workspace: rns_kv_attention_workspace() bytes of scratch of the
  * caller's stream, 16-byte aligned; nothing in it has to be initialised.  A call launches two to
  * four kernels over it: host threads that share a stream do not share a workspace, or make their
  * calls one after the other.

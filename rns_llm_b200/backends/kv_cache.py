@@ -106,7 +106,8 @@ class KVCacheOperators:
         and become the last tokens of its ``seq_lens[b]`` (int32 [sequences], the lengths AFTER the
         write).  ``page_table`` int32 [sequences, pages per sequence].  A page that already holds
         tokens of the sequence is rescaled when a larger value arrives.  ``max_query_len`` bounds
-        the new tokens of one sequence (default: all tokens)."""
+        the new tokens of one sequence (default: all tokens); one that has more is reported and not
+        written."""
         if k.ndim != 3 or k.shape != v.shape or k.shape[1] != cache.kv_heads or k.shape[2] != cache.head_dim:
             raise ValueError("k and v must be [tokens, kv_heads, head_dim] of the cache")
         if k.dtype not in _FLOAT_TYPES or v.dtype != k.dtype:
@@ -133,7 +134,8 @@ class KVCacheOperators:
 
         Rows ``row_starts[b]:row_starts[b+1]`` (int32 [sequences+1]) are sequence b's tokens from
         position ``first[b]`` (int32 [sequences]) on; rows behind the last sequence's are not
-        written.  ``max_rows`` bounds the rows of one sequence (default: all rows)."""
+        written.  ``max_rows`` bounds the rows of one sequence (default: all rows); one that has more
+        is reported and not read."""
         rows = int(rows)
         if rows < 0:
             raise ValueError("rows must not be negative")
@@ -172,7 +174,10 @@ class KVCacheOperators:
         nothing gets zeros.  Rows of no sequence are not written.  ``out``, where given, shares no
         element with ``q``.  Returns the output in q's type
         and, with ``return_lse``, also float32 [tokens, heads]: the log of the sum of the
-        exponentials of the scaled scores (-inf where nothing is seen)."""
+        exponentials of the scaled scores (-inf where nothing is seen).
+
+        ``max_query_len`` bounds the new tokens of one sequence and chooses the kernels by it; without
+        it a decode step of many sequences counts as one of many new tokens, which costs time."""
         if q.ndim != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.kv_heads or q.shape[1] == 0:
             raise ValueError("q must be [tokens, heads, head_dim] with heads a multiple of the cache's kv_heads")
         if q.dtype != torch.float16 and q.dtype != torch.bfloat16:

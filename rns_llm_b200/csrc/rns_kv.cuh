@@ -1,5 +1,6 @@
-// Paged 8-bit key/value cache: addressing and checks shared by rns_kv_sm100.cu and
-// rns_kv_attention_sm100.cu.
+// Paged 8-bit key/value cache: addressing, checks and conversions shared by the files that write and read it
+// (rns_kv_sm100.cu) and attend to it (rns_kv_attention_sm100.cu and its kernels, rns_kv_decode_sm100.cu and
+// rns_kv_prompt_sm100.cu).
 //
 // A cache holds `pages` pages; page p of head h is `page_tokens` rows of `head_dim` bytes at
 // ((p * kv_heads + h) * page_tokens) * head_dim of d_k and d_v, and its values stand for

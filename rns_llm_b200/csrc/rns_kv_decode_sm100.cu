@@ -31,9 +31,9 @@
 //   rescaling is exact, and follows the row's own scores and their pages' scales alone: what a row
 //   gives does not depend on the rows beside it.
 //
-// Measured (graph replay): 64 sequences of 1..8192 tokens, 32 over 8 heads of 128, 145 us = 3.70 TB/s of cache
+// Measured (graph replay): 64 sequences of 1..8192 tokens, 32 over 8 heads of 128, 145 us = 3.7 TB/s of cache
 // (0.57 of the copy rate; about 470 instructions for 16 keys, issue slots 53 % busy with three warps a scheduler: the
-// latency of dependent instructions bounds it); one sequence of 131072, e4m3, 69 us; 8 of 640, 12 heads of 64, 16 us.
+// latency of dependent instructions bounds it); one sequence of 131072, e4m3, 70 us; 8 of 640, 12 heads of 64, 16 us.
 #include "rns_kv.cuh"
 #include "rns_ptx.cuh"
 

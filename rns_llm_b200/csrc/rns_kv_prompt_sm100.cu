@@ -25,12 +25,13 @@
 // * Work is cut as there: one axis of key blocks over all items, equal shares, pieces joined by a
 //   second kernel.
 //
-// Measured (graph replay): a chunk of 509 tokens behind 32768, 32 over 8 heads of 128, 328 us = 840 TFLOP/s; a
-// prompt of 4096 tokens of 32 heads 229 us; 8 prompts of 512 of 12 heads of 64 38 us.  In steady state a block
-// of both tiles takes 4850 cycles, 2048 of them on the tensor pipe: what bounds it is the chain of one tile,
-// scores -> 430 cycles for the largest -> 2250 for the weights -> second product -> next scores.
-// Heads of 256, where nothing overlaps that chain: a prompt of 2048 tokens of 16 heads 130 us (653 in the rows
-// kernel), 509 tokens behind 8192, 16 over 4 heads, 166 us = 424 TFLOP/s (570 in the rows kernel).
+// Measured (graph replay): a chunk of 509 tokens behind 32768, 32 over 8 heads of 128, 335 us = 823 TFLOP/s; a
+// prompt of 4096 tokens of 32 heads 236 us; 8 prompts of 512 of 12 heads of 64 39 us.  In steady state a block
+// of both tiles takes 4850 cycles (counted when the chunk took 328 us), 2048 of them on the tensor pipe: what
+// bounds it is the chain of one tile, scores -> 430 cycles for the largest -> 2250 for the weights -> second
+// product -> next scores.
+// Heads of 256, where nothing overlaps that chain: a prompt of 2048 tokens of 16 heads 128 us (653 in the rows
+// kernel), 509 tokens behind 8192, 16 over 4 heads, 165 us = 426 TFLOP/s (570 in the rows kernel).
 //
 // Warps 0-3 and 4-7: softmax of a tile, a thread a row (the same warps fetch the queries and store the
 // outputs); 8-11: conversion; 12: issues the products; 13: copies; 14: scales of the pages; 15: the list of
@@ -48,8 +49,8 @@ constexpr float kNoScore = -1.7e38f;      // below every score: "nothing seen ye
 constexpr float kScoreLag = 8.0f;
 constexpr int kScaleSlots = 4, kPartSlots = 4;
 // What starting and ending an item costs, in blocks: each item takes that much more of the axis that is shared
-// out (prompt of 4096 tokens, 32 heads: 245 us without, 227 / 229 / 234 with 2 / 3 / 5; 8 prompts of 512: 42.2
-// without, 39.0 / 38.4 / 37.1).
+// out (prompt of 4096 tokens, 32 heads, when it took 229 us: 245 us without, 227 / 229 / 234 with 2 / 3 / 5; 8
+// prompts of 512: 42.2 without, 39.0 / 38.4 / 37.1).
 constexpr int kItemCost = 3;
 // Registers: a softmax thread holds its row's scores of a block.  8 warps of kSoftmaxRegs and 8 of kOtherRegs
 // must not exceed what the block was launched with, 16 warps of kLaunchRegs (build.py refuses to build the kernel
@@ -273,10 +274,10 @@ __device__ __forceinline__ uint32_t half_pair_e4m3(uint32_t x) {
     return r;
 }
 
-// Waits of whole warps, bounded by about a second of SM clock.  A poll may sleep for up to 0.1 ms until
-// its phase completes: most of 24 warps wait at any time, and without a time to sleep their polls took
-// more issue slots than the work.  Waits are kept small, too: eight different programs share the
-// instruction cache.
+// Waits of whole warps, bounded by about a second of SM clock.  A poll may be suspended for up to 0.1 ms until
+// its phase completes, as most of the 16 warps wait at any time (with the hardware's own limit instead, the chunk
+// takes 332 us for 333, a prompt of 4096 tokens 237 for 237).  Waits are kept small: six different programs share
+// the instruction cache.
 __device__ __forceinline__ bool prompt_poll(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -346,7 +347,7 @@ __device__ __forceinline__ float prompt_top(uint32_t s_tmem, const PromptScales&
 }
 // Scores -> 2^(s f + exponent - m), whose sum without the exponents is returned, and times the values' weight as
 // fp16 into the place of the scores.  A loop over 32 columns, read a second time, rather than 128 held and unrolled: the code of all
-// eight programs has to stay in the instruction caches.  The next columns are fetched as soon as the
+// six programs has to stay in the instruction caches.  The next columns are fetched as soon as the
 // multiply-adds have taken these.
 __device__ __forceinline__ float prompt_weights(uint32_t s_tmem, const PromptScales& sc, float q_scale, float m) {
     Pair sums[4] = {0, 0, 0, 0};                                    // independent: the additions must not wait for one another
