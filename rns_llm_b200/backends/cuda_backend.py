@@ -260,7 +260,7 @@ class CudaRNSBackend(KVCacheOperators):
                 wait_info=torch.zeros(4, dtype=torch.int32, device=dev),
                 histogram=torch.zeros(N.MAX_CHANNELS + 1, dtype=torch.int64, device=dev),
             )
-            self._device_state[index] = state
+            state = self._device_state.setdefault(index, state)      # (another thread's, if it was first)
         return state
 
     def reset_stats(self) -> None:

@@ -1,4 +1,6 @@
-"""Captured calls of the quantised cache on the GPU: first calls and status."""
+"""Captured calls of the quantised cache on the GPU, first calls and status, and calls of several host threads."""
+import threading
+
 import pytest
 import torch
 
@@ -69,4 +71,46 @@ def test_first_call_of_a_backend_is_not_captured():
     with torch.cuda.graph(graph):
         backend.kv_cache_write(cache, x, x, *args)
     graph.replay()
+    backend.check_status()
+
+
+def test_host_threads_on_one_stream():
+    """Attention whose keys are split among CTAs, of two kernels in turn, beside a linear that uses the same scratch:
+    every result is that of a call alone."""
+    from rns_llm_b200.backends import CudaRNSBackend
+    from rns_llm_b200.layers import RNSLinear
+
+    backend = CudaRNSBackend()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+
+    def attention(new, length):
+        cache = backend.create_kv_cache(pages=64, kv_heads=2, head_dim=64, page_tokens=64)
+        table, lens, starts = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64), ints(length), ints(0, length)
+        x = torch.randn(length, 2, 64, generator=gen, device="cuda").half()
+        backend.kv_cache_write(cache, x, x, table, lens, starts)
+        q = torch.randn(new, 4, 64, generator=gen, device="cuda").half()
+        return lambda: backend.kv_cache_attention(q, cache, table, lens, ints_like(starts, (0, new)))
+
+    linear = RNSLinear.from_linear(torch.nn.Linear(2048, 512, device="cuda", dtype=torch.float16), backend=backend,
+                                   mode="rns", fused=True, moduli=(127, 126, 125, 121)).eval()
+    rows = torch.randn(64, 2048, generator=gen, device="cuda").half()
+    calls = [attention(1, 4000), attention(70, 3500), attention(3, 4096), lambda: linear(rows)]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    outs, started = [[] for _ in calls], threading.Barrier(len(calls))
+
+    def work(i):
+        started.wait()
+        with torch.no_grad():
+            for _ in range(60):
+                outs[i].append(calls[i]())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    for got, alone in zip(outs, want):
+        assert len(got) == 60 and all(torch.equal(out, alone) for out in got)
     backend.check_status()
