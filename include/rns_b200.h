@@ -635,18 +635,19 @@ RNS_API int rns_kv_read(const rns_kv_cache* cache, const int32_t* d_first, const
  * j > p - window when window > 0 (window needs causal).  A query that sees nothing (p < 0, more
  * queries than tokens or an empty sequence, included) gets zeros.
  *   d_q    [tokens, heads, head_dim] F16 or BF16, strides in elements, unit inner stride
- *   d_out  [tokens, heads, head_dim] of q's type, likewise; rows of no sequence stay as they are
+ *   d_out  [tokens, heads, head_dim] of q's type, likewise, sharing no element with d_q; rows of no
+ *          sequence stay as they are
  *   d_lse  float [tokens, heads] or NULL: log of the sum of exp of the scaled scores (-inf where
  *          a query sees nothing)
- * Scores, softmax and sums are fp32.  A softmax weight p_j meets the values off by 2^-22 of itself
- * (2^-11 in calls with a sequence of more than 32 query rows, new tokens x heads that share one of
- * the cache's), or by 2^-24 of the row's largest product of a weight and its page's value scale, if
- * that is more.
+ * Scores, softmax and sums are fp32 (a scaled score below -1e38 counts as not seen).  A softmax
+ * weight p_j meets the values off by 2^-22 of itself (2^-11 in calls with a sequence of more than 32
+ * query rows, new tokens x heads that share one of the cache's), or by 2^-24 of the row's largest
+ * product of a weight and its page's value scale, if that is more.
  * max_new: no sequence of the call has more new tokens.  It only chooses kernels and tiles here: one
- * that is too small or far too large costs time, not results.  d_workspace: rns_kv_attention_workspace() bytes of scratch of the
- * caller's stream, 16-byte aligned; nothing in it has to be initialised.  A call launches two to
- * four kernels over it: host threads that share a stream do not share a workspace, or make their
- * calls one after the other.
+ * that is too small or far too large costs time, not results.
+ * d_workspace: rns_kv_attention_workspace() bytes of scratch of the caller's stream, 16-byte aligned;
+ * nothing in it has to be initialised.  A call launches two to four kernels over it: host threads
+ * that share a stream do not share a workspace, or make their calls one after the other.
  */
 typedef struct rns_kv_attention_args {
     const void* d_q;
