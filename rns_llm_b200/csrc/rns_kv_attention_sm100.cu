@@ -3,7 +3,8 @@
 // One pass over the keys a query sees, with the running maximum m and sum l of the softmax:
 //     t_j = scale * s_k * (q . k_j) / ln 2,   m' = max(m, t),   l' = l 2^(m - m') + sum 2^(t_j - m')
 //     o'  = o 2^(m - m') + sum 2^(t_j - m') s_v v_j
-// and out = o / l, lse = (m + log2 l) ln 2.
+// and out = o / l, lse = (m + log2 l) ln 2.  The kernels take m near the largest t + log2 s_v, so that o's weights
+// with their scales stay in fp16's range (kv_value_scale); any m gives the same out and lse.
 #include "rns_kv.cuh"
 
 #include <cmath>
@@ -38,7 +39,7 @@ static int check_attention(const rns_kv_cache* cache, const rns_kv_attention_arg
 
 // Which kernel serves which sequences: tiles of the rows kernel hold up to 32 query rows (new tokens x
 // heads that share one of the cache), those of the prompt kernel 256 (128 of heads above 128).  Beyond 32 rows
-// the rows kernel reads a sequence's keys once for every tile (8 prompts of 512: 182 us there, 38 us in the
+// the rows kernel reads a sequence's keys once for every tile (8 prompts of 512: 182 us there, 39 us in the
 // prompt kernel; 48 rows of heads of 256, four sequences of 8000 tokens: 83 and 70 us).
 struct Routing {
     bool rows, prompt;
